@@ -221,6 +221,64 @@ B200EP_API int b200ep_paged_attention(const b200ep_paged_params* p, const void* 
                                       const int32_t* block_table, const void* cos_cache,
                                       const void* sin_cache, void* out, int dtype, void* stream);
 
+/* 8-bit paged KV cache ------------------------------------------------------------------------
+ * No counterpart in the reference, whose caches hold the I/O type: half the bytes of PagedAttention's
+ * caches, with one fp32 scale per token and kv head.
+ *   key_cache, value_cache    codes [num_blocks, kv_heads, block_size, head_size], int8 or
+ *                             float8e4m3fn (cache_type), 16-byte aligned
+ *   key_scales, value_scales  float32 [num_blocks, kv_heads, block_size]
+ * A row is held as code * scale with scale = max|x| / 127 (int8) or / 448 (float8e4m3fn) and
+ * code = x / scale rounded to nearest, ties to even; a row of zeros has scale 0, and a row that holds
+ * an infinity or a NaN reads back as NaN.  Packed rows, cumulative_seqlens, past_seqlens, block_table
+ * and the cos / sin caches are those of b200ep_paged_attention (a page of -1 or outside the cache, a
+ * position outside the table or the cos / sin rows: the row is skipped and the device error word set).
+ * dtype (of rows, cos / sin and outputs): float32, float16 or bfloat16.  head_size 32, 64, 128 or 256;
+ * any block_size. */
+typedef struct b200ep_paged_q8_params {
+  int32_t batch;       /* sequences: cumulative_seqlens has batch + 1 entries */
+  int32_t num_tokens;  /* packed rows (= cumulative_seqlens[batch]) */
+  int32_t num_heads, kv_heads, head_size;
+  int32_t num_blocks, block_size, max_blocks; /* caches' pages, rows per page; block_table row */
+  int32_t max_seq, rotary_half;               /* cos/sin cache rows and columns (do_rotary) */
+  int32_t do_rotary, interleaved;
+  int32_t cache_type;                         /* 3: int8, 17: float8e4m3fn */
+  float scale;                                /* 0: 1/sqrt(head_size) */
+  int64_t query_stride, key_stride, value_stride; /* elements from row to row (slices of a packed
+                                                     projection); 0: heads * head_size */
+} b200ep_paged_q8_params;
+
+/* Writes new key rows (RoPE'd at their positions when do_rotary, in fp32) and value rows
+ * [num_tokens, kv_heads * head_size] into their pages. */
+B200EP_API int b200ep_paged_kv_quantize(const b200ep_paged_q8_params* p, const void* key, const void* value,
+                                        void* key_cache, void* value_cache, float* key_scales,
+                                        float* value_scales, const int32_t* cumulative_seqlens,
+                                        const int32_t* past_seqlens, const int32_t* block_table,
+                                        const void* cos_cache, const void* sin_cache, int dtype, void* stream);
+
+/* Reads the first seqlens[b] positions of each sequence into key / value [batch, kv_heads, cap,
+ * head_size] (the shared-buffer layout of b200ep_group_query_attention, whose prompt kernels can then
+ * attend to them); positions from seqlens[b] to cap are set to zero.  Outputs 16-byte aligned. */
+B200EP_API int b200ep_paged_kv_dequantize(const b200ep_paged_q8_params* p, const void* key_cache,
+                                          const void* value_cache, const float* key_scales,
+                                          const float* value_scales, const int32_t* seqlens,
+                                          const int32_t* block_table, void* key, void* value, int64_t cap,
+                                          int dtype, void* stream);
+
+/* Attention over the 8-bit cache.  Row j of sequence b sees positions 0 .. past_seqlens[b] + j; its
+ * query is RoPE'd here.  With key / value (both, or neither) the new rows are first written as by
+ * b200ep_paged_kv_quantize.  out [num_tokens, num_heads * head_size].  Meant for one or a few new
+ * tokens per sequence: every row reads its keys on its own, so a long prompt is better attended by
+ * reading its past back (b200ep_paged_kv_dequantize) and b200ep_group_query_attention.
+ * workspace: b200ep_paged_attention_quantized_workspace_size(p) bytes (num_heads, kv_heads and
+ * head_size are looked at), 16-byte aligned, contents irrelevant; calls that may overlap on the GPU
+ * need workspaces of their own. */
+B200EP_API size_t b200ep_paged_attention_quantized_workspace_size(const b200ep_paged_q8_params* p);
+B200EP_API int b200ep_paged_attention_quantized(
+    const b200ep_paged_q8_params* p, const void* query, const void* key, const void* value, void* key_cache,
+    void* value_cache, float* key_scales, float* value_scales, const int32_t* cumulative_seqlens,
+    const int32_t* past_seqlens, const int32_t* block_table, const void* cos_cache, const void* sin_cache,
+    void* out, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

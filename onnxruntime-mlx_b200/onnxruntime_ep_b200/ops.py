@@ -35,6 +35,17 @@ class PagedParams(ctypes.Structure):
     ]
 
 
+class PagedQ8Params(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("num_tokens", ctypes.c_int32), ("num_heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("head_size", ctypes.c_int32), ("num_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32), ("max_blocks", ctypes.c_int32), ("max_seq", ctypes.c_int32),
+        ("rotary_half", ctypes.c_int32), ("do_rotary", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("cache_type", ctypes.c_int32), ("scale", ctypes.c_float), ("query_stride", ctypes.c_int64),
+        ("key_stride", ctypes.c_int64), ("value_stride", ctypes.c_int64),
+    ]
+
+
 _configured = False
 
 
@@ -60,6 +71,12 @@ def _lib():
         L.b200ep_gqa_sliding_workspace_size.restype = ctypes.c_size_t
         L.b200ep_group_query_attention_sliding.argtypes = (
             [ctypes.POINTER(GqaParams)] + [vp] * 11 + [i32, vp, ctypes.c_size_t, vp])
+        q8 = ctypes.POINTER(PagedQ8Params)
+        L.b200ep_paged_kv_quantize.argtypes = [q8] + [vp] * 11 + [i32, vp]
+        L.b200ep_paged_kv_dequantize.argtypes = [q8] + [vp] * 8 + [i64, i32, vp]
+        L.b200ep_paged_attention_quantized_workspace_size.argtypes = [q8]
+        L.b200ep_paged_attention_quantized_workspace_size.restype = ctypes.c_size_t
+        L.b200ep_paged_attention_quantized.argtypes = [q8] + [vp] * 13 + [i32, vp, ctypes.c_size_t, vp]
         _configured = True
     return L
 
@@ -242,4 +259,153 @@ def paged_attention(query, key, value, key_cache, value_cache, cumulative_seqlen
         ctypes.byref(p), _p(query), _p(key), _p(value), _p(key_cache), _p(value_cache), _p(cumulative_seqlens),
         _p(past_seqlens), _p(block_table), _p(cos_cache), _p(sin_cache), _p(out), _dt(query),
         _stream(query.device)))
+    return out
+
+
+def _q8_params(key_cache, value_cache, key_scales, value_scales, block_table, batch, cos_cache=None, interleaved=0):
+    """The cache's geometry, checked the way the kernels rely on it."""
+    import torch
+
+    types = {torch.int8: 3, torch.float8_e4m3fn: 17}
+    if key_cache.dtype not in types or value_cache.dtype != key_cache.dtype:
+        raise ValueError("paged 8-bit cache: key_cache and value_cache must both be int8 or float8_e4m3fn")
+    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
+        raise ValueError("paged 8-bit cache: caches must be [num_blocks, kv_heads, block_size, head_size]")
+    for s in (key_scales, value_scales):
+        if s.dtype != torch.float32 or s.shape != key_cache.shape[:3]:
+            raise ValueError("paged 8-bit cache: scales must be float32 [num_blocks, kv_heads, block_size]")
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous() and key_scales.is_contiguous()
+            and value_scales.is_contiguous()):
+        raise ValueError("paged 8-bit cache: caches and scales must be contiguous")
+    if block_table.dtype != torch.int32 or not block_table.is_contiguous() or (
+            batch and block_table.numel() % batch):
+        raise ValueError("paged 8-bit cache: block_table must be a contiguous int32 [batch, max_blocks]")
+    p = PagedQ8Params()
+    p.num_blocks, p.kv_heads, p.block_size, p.head_size = key_cache.shape
+    p.batch = batch
+    p.max_blocks = block_table.numel() // batch if batch else 1
+    p.cache_type = types[key_cache.dtype]
+    if cos_cache is not None:
+        p.do_rotary, p.interleaved = 1, int(interleaved)
+        p.max_seq, p.rotary_half = cos_cache.shape
+    return p
+
+
+def _q8_rows(name, x, width, dtype=None, tokens=None):
+    """Packed rows [T, width]; the rows may be slices of wider ones.  Returns the row stride."""
+    if x.dim() != 2 or x.shape[1] != width or (tokens is not None and x.shape[0] != tokens):
+        raise ValueError(f"paged 8-bit cache: {name} must be [{'T' if tokens is None else tokens}, {width}]")
+    if dtype is not None and x.dtype != dtype:
+        raise ValueError(f"paged 8-bit cache: {name} must be {dtype}")
+    if x.shape[0] > 1 and (x.stride(1) != 1 or x.stride(0) < width) or x.shape[0] == 1 and x.stride(1) != 1:
+        raise ValueError(f"paged 8-bit cache: the elements of a row of {name} must be contiguous")
+    return x.stride(0) if x.shape[0] > 1 else width
+
+
+def _q8_control(cumulative_seqlens, past_seqlens, cos_cache, sin_cache, dtype):
+    import torch
+
+    for name, t in (("cumulative_seqlens", cumulative_seqlens), ("past_seqlens", past_seqlens)):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"paged 8-bit cache: {name} must be contiguous int32")
+    if cumulative_seqlens.numel() != past_seqlens.numel() + 1:
+        raise ValueError("paged 8-bit cache: cumulative_seqlens must have one entry more than past_seqlens")
+    if (cos_cache is None) != (sin_cache is None):
+        raise ValueError("paged 8-bit cache: cos_cache and sin_cache come together")
+    if cos_cache is not None:
+        for t in (cos_cache, sin_cache):
+            if t.dtype != dtype or t.shape != cos_cache.shape or t.dim() != 2 or not t.is_contiguous():
+                raise ValueError("paged 8-bit cache: cos / sin must be contiguous [max_seq, rotary_half] of the "
+                                 "rows' type")
+
+
+def paged_kv_quantize(key, value, key_cache, value_cache, key_scales, value_scales, cumulative_seqlens,
+                      past_seqlens, block_table, cos_cache=None, sin_cache=None, *, interleaved=0):
+    """Write packed key / value rows [T, kv_heads * D] (the key after RoPE) into 8-bit pages, in place:
+    codes [num_blocks, kv_heads, block_size, D] int8 or float8_e4m3fn, scales float32
+    [num_blocks, kv_heads, block_size].  Rows may be slices of a packed projection."""
+    p = _q8_params(key_cache, value_cache, key_scales, value_scales, block_table, past_seqlens.numel(), cos_cache,
+                   interleaved)
+    _q8_control(cumulative_seqlens, past_seqlens, cos_cache, sin_cache, key.dtype)
+    width = p.kv_heads * p.head_size
+    p.key_stride = _q8_rows("key", key, width)
+    p.value_stride = _q8_rows("value", value, width, key.dtype, key.shape[0])
+    p.num_tokens = key.shape[0]
+    check(_lib().b200ep_paged_kv_quantize(
+        ctypes.byref(p), _p(key), _p(value), _p(key_cache), _p(value_cache), _p(key_scales), _p(value_scales),
+        _p(cumulative_seqlens), _p(past_seqlens), _p(block_table), _p(cos_cache), _p(sin_cache), _dt(key),
+        _stream(key.device)))
+
+
+def paged_kv_dequantize(key_cache, value_cache, key_scales, value_scales, seqlens, block_table, *, cap=None,
+                        dtype=None, key=None, value=None):
+    """Read the first seqlens[b] positions of each sequence out of 8-bit pages: (key, value), each
+    [B, kv_heads, cap, D] of ``dtype`` with zeros from seqlens[b] on — GroupQueryAttention's shared-buffer
+    layout.  ``cap`` and ``dtype`` are taken from ``key`` / ``value`` when those are given."""
+    import torch
+
+    B = seqlens.numel()
+    p = _q8_params(key_cache, value_cache, key_scales, value_scales, block_table, B)
+    if seqlens.dtype != torch.int32 or not seqlens.is_contiguous():
+        raise ValueError("paged 8-bit cache: seqlens must be contiguous int32")
+    if (key is None) != (value is None):
+        raise ValueError("paged 8-bit cache: key and value come together")
+    if key is None:
+        if cap is None:
+            raise ValueError("paged 8-bit cache: cap is needed when no output is given")
+        shape = (B, p.kv_heads, cap, p.head_size)
+        key = torch.empty(shape, dtype=dtype or torch.float16, device=key_cache.device)
+        value = torch.empty_like(key)
+    else:
+        cap = key.shape[2] if key.dim() == 4 else -1
+        if key.shape != (B, p.kv_heads, cap, p.head_size) or value.shape != key.shape or (
+                value.dtype != key.dtype) or not (key.is_contiguous() and value.is_contiguous()):
+            raise ValueError("paged 8-bit cache: outputs must be contiguous [B, kv_heads, cap, D] of one type")
+    check(_lib().b200ep_paged_kv_dequantize(
+        ctypes.byref(p), _p(key_cache), _p(value_cache), _p(key_scales), _p(value_scales), _p(seqlens),
+        _p(block_table), _p(key), _p(value), cap, _dt(key), _stream(key.device)))
+    return key, value
+
+
+def paged_attention_quantized_workspace_size(*, num_heads, kv_heads, head_size) -> int:
+    p = PagedQ8Params()
+    p.num_heads, p.kv_heads, p.head_size = num_heads, kv_heads, head_size
+    return int(_lib().b200ep_paged_attention_quantized_workspace_size(ctypes.byref(p)))
+
+
+def paged_attention_quantized(query, key, value, key_cache, value_cache, key_scales, value_scales,
+                              cumulative_seqlens, past_seqlens, block_table, cos_cache=None, sin_cache=None, *,
+                              num_heads, kv_heads, scale=0.0, interleaved=0, out=None, workspace=None):
+    """PagedAttention over 8-bit pages (see paged_kv_quantize): packed query rows [T, num_heads * D], RoPE'd
+    here, each attending to its sequence's positions up to its own.  ``key`` / ``value`` (both or neither)
+    are first written into the pages.  ``workspace``: a uint8 tensor of at least
+    paged_attention_quantized_workspace_size bytes, any contents; allocated on the current stream when
+    absent."""
+    import torch
+
+    p = _q8_params(key_cache, value_cache, key_scales, value_scales, block_table, past_seqlens.numel(), cos_cache,
+                   interleaved)
+    _q8_control(cumulative_seqlens, past_seqlens, cos_cache, sin_cache, query.dtype)
+    if p.kv_heads != kv_heads:
+        raise ValueError(f"paged 8-bit cache: the cache holds {p.kv_heads} kv heads, not {kv_heads}")
+    T, D = query.shape[0], p.head_size
+    p.num_heads, p.num_tokens, p.scale = num_heads, T, float(scale)
+    p.query_stride = _q8_rows("query", query, num_heads * D)
+    if (key is None) != (value is None):
+        raise ValueError("paged 8-bit cache: key and value come together, or neither")
+    if key is not None:
+        p.key_stride = _q8_rows("key", key, kv_heads * D, query.dtype, T)
+        p.value_stride = _q8_rows("value", value, kv_heads * D, query.dtype, T)
+    if out is None:
+        out = torch.empty(T, num_heads * D, dtype=query.dtype, device=query.device)
+    elif out.shape != (T, num_heads * D) or out.dtype != query.dtype or not out.is_contiguous():
+        raise ValueError("paged 8-bit cache: out must be contiguous [T, num_heads * D] of the query's type")
+    L = _lib()
+    if workspace is None:
+        workspace = torch.empty(L.b200ep_paged_attention_quantized_workspace_size(ctypes.byref(p)),
+                                dtype=torch.uint8, device=query.device)
+    check(L.b200ep_paged_attention_quantized(
+        ctypes.byref(p), _p(query), _p(key), _p(value), _p(key_cache), _p(value_cache), _p(key_scales),
+        _p(value_scales), _p(cumulative_seqlens), _p(past_seqlens), _p(block_table), _p(cos_cache), _p(sin_cache),
+        _p(out), _dt(query), _p(workspace), workspace.numel() * workspace.element_size(), _stream(query.device)))
     return out
