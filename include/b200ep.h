@@ -279,6 +279,23 @@ B200EP_API int b200ep_paged_attention_quantized(
     const int32_t* past_seqlens, const int32_t* block_table, const void* cos_cache, const void* sin_cache,
     void* out, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Token sampling ------------------------------------------------------------------------------
+ * One token per row of logits [rows, vocab] (dtype; row stride in elements, 0 = vocab).  No counterpart in the
+ * reference.  With w_j = exp((x_j - max x) / temperature) and tokens ordered by logit (ties: lowest index
+ * first), kept are the first top_k; of these, those with less than top_p of the top_k's mass before them;
+ * of these, those with w_j >= min_p; always the first.  The token is the kept one with the largest
+ * w_j / noise_j (ties: lowest index): for noise of independent standard exponential numbers (float32
+ * [rows, vocab], > 0) that is a draw from the kept tokens' distribution.
+ *   temperature [rows]: 0 takes the first token (NULL: 1);  top_k int32 [rows]: <= 0 keeps all (NULL);
+ *   top_p [rows]: >= 1 keeps all (NULL);  min_p [rows]: <= 0 keeps all (NULL)
+ *   tokens int64 [rows]: -1 for a row without a logit above -infinity;  logprobs float32 [rows] (may be
+ *   NULL): log softmax of the logits as given, at the token
+ * NaN logits are never taken.  Equal inputs give equal tokens.  vocab up to 262144. */
+B200EP_API int b200ep_sample(const void* logits, const float* noise, const float* temperature,
+                             const int32_t* top_k, const float* top_p, const float* min_p, int64_t* tokens,
+                             float* logprobs, int64_t rows, int64_t vocab, int64_t logits_stride,
+                             int64_t noise_stride, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

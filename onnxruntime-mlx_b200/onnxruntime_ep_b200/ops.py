@@ -77,6 +77,7 @@ def _lib():
         L.b200ep_paged_attention_quantized_workspace_size.argtypes = [q8]
         L.b200ep_paged_attention_quantized_workspace_size.restype = ctypes.c_size_t
         L.b200ep_paged_attention_quantized.argtypes = [q8] + [vp] * 13 + [i32, vp, ctypes.c_size_t, vp]
+        L.b200ep_sample.argtypes = [vp] * 8 + [i64] * 4 + [i32, vp]
         _configured = True
     return L
 
@@ -409,3 +410,36 @@ def paged_attention_quantized(query, key, value, key_cache, value_cache, key_sca
         _p(value_scales), _p(cumulative_seqlens), _p(past_seqlens), _p(block_table), _p(cos_cache), _p(sin_cache),
         _p(out), _dt(query), _p(workspace), workspace.numel() * workspace.element_size(), _stream(query.device)))
     return out
+
+
+def sample(logits, noise, temperature=None, top_k=None, top_p=None, min_p=None, *, tokens=None, logprobs=None):
+    """Draw one token per row of ``logits`` [B, V]: (tokens int64 [B], logprobs float32 [B]).  ``noise``: float32
+    [B, V] of standard exponential numbers (``torch.empty(B, V).exponential_()``).  ``temperature`` (0: the largest
+    logit), ``top_k`` int32 (<= 0: all), ``top_p`` (>= 1: all) and ``min_p`` (<= 0: all) are [B] or None.  Rows may
+    be slices of wider ones.  tokens is -1 where every logit is -inf or NaN."""
+    import torch
+
+    if logits.dim() != 2 or noise.shape != logits.shape:
+        raise ValueError("sample: logits and noise must both be [B, V]")
+    if noise.dtype != torch.float32:
+        raise ValueError("sample: noise must be float32")
+    B, V = logits.shape
+    for name, x in (("logits", logits), ("noise", noise)):
+        if V > 1 and x.stride(1) != 1 or B > 1 and x.stride(0) < V:
+            raise ValueError(f"sample: the elements of a row of {name} must be contiguous")
+    for name, x, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if x is not None and (x.dtype != dtype or x.shape != (B,) or not x.is_contiguous()):
+            raise ValueError(f"sample: {name} must be contiguous {dtype} [{B}]")
+    if tokens is None:
+        tokens = torch.empty(B, dtype=torch.int64, device=logits.device)
+    elif tokens.dtype != torch.int64 or tokens.numel() != B or not tokens.is_contiguous():
+        raise ValueError(f"sample: tokens must be contiguous int64 with {B} entries")
+    if logprobs is None:
+        logprobs = torch.empty(B, dtype=torch.float32, device=logits.device)
+    elif logprobs.dtype != torch.float32 or logprobs.shape != (B,) or not logprobs.is_contiguous():
+        raise ValueError(f"sample: logprobs must be contiguous float32 [{B}]")
+    check(_lib().b200ep_sample(_p(logits), _p(noise), _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(tokens),
+                               _p(logprobs), B, V, logits.stride(0) if B > 1 else 0, noise.stride(0) if B > 1 else 0,
+                               _dt(logits), _stream(logits.device)))
+    return tokens, logprobs
