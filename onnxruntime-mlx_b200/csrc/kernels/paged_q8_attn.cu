@@ -36,34 +36,33 @@ namespace b200ep {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kUnit = 32;  // keys of a unit
-constexpr int kLift = 14;  // P vs is held times 2^kLift
+constexpr int kThreads = kWarps * 32;
+constexpr int kLift = 6;       // P vs is held times 2^kLift
+constexpr float kSlack = 8.f;  // a score may pass the running maximum by this much (in base 2) before it moves
 
-template <int D, int NT>
+template <typename T, int D, int NT>
 struct Cfg {
-  static constexpr int kStages = D >= 256 ? 3 : D == 128 ? 3 : 4;
-  static constexpr int kCtasPerSm = D >= 256 || (D == 128 && NT == 2) ? 1 : 2;
-  static constexpr int kHeads = 8 * NT;
-  static constexpr int kData = kUnit * D;                          // K (or V) codes of a unit
-  static constexpr int kStageBytes = 2 * kData + 2 * kUnit * 4;    // K, V, ks, vs
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kMerge = kRing;                             // [2][kHeads][D + 4] fp32 (two warps at a time)
-  static constexpr int kMl = kMerge + 2 * kHeads * (D + 4) * 4;    // [kWarps][kHeads][2] fp32
-  static constexpr int kMeta = kMl + kWarps * kHeads * 2 * 4;      // [kWarps][kStages] Meta
-  static constexpr int kTotal = kMeta + kWarps * kStages * 32;
+  static constexpr int kNQ = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;  // fp16 terms of q
+  static constexpr int kNP = std::is_same<T, float>::value ? 2 : 1;          // fp16 terms of P
+  static constexpr int kUnit = 16 * NT;  // keys of a unit
+  static constexpr int kHeads = 8 * NT;  // query heads of a CTA
+  static constexpr int kStages = D >= 128 ? 3 : D == 64 ? 5 : 8;
+  static constexpr int kCtasPerSm = D == 256 || NT == 2 ? 2 : std::is_same<T, float>::value ? 3 : 4;
+  static constexpr int kData = kUnit * D;                         // K (or V) codes of a unit
+  static constexpr int kStageBytes = 2 * kData + 2 * kUnit * 4;   // K, V, ks, vs; holds [kHeads][D] fp32 at a merge
+  static constexpr int kQ = kWarps * kStages * kStageBytes;       // the query operand
+  static constexpr int kQBytes = kNQ * NT * (D / 16) * 32 * 8;
+  static constexpr int kMl = kQ + kQBytes;                        // [kWarps][kHeads] (m, l)
+  static constexpr int kScale = kMl + kWarps * kHeads * 8;        // [kHeads] score factor
+  static constexpr int kMisc = kScale + kHeads * 4;               // [kWarps] (output factor, buffer)
+  static constexpr int kTotal = kMisc + kWarps * 8;
 };
 
-struct Meta {  // what a streamed unit is
-  int row, hc, u, n;
-  uint32_t valid;
-  int pad[3];
-};
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -165,9 +164,17 @@ __device__ __forceinline__ float q_at(const T* x, int d, const PagedQ8& kp, int 
 
 // Keys that row i sees (0: none, an invalid row) and its sequence.
 __device__ __forceinline__ int row_keys(const PagedQ8& kp, int i, int& seq) {
-  seq = i < kp.ntok ? q8_seq(kp.cum, kp.batch, i) : -1;
-  if (seq < 0) return 0;
-  const int pos = __ldg(kp.past + seq) + (i - __ldg(kp.cum + seq));
+  seq = -1;
+  if (i >= kp.ntok) return 0;
+  int past = i < kp.batch ? __ldg(kp.past + i) : 0, first = i;  // (one new token per sequence: row i is sequence i)
+  if (i < kp.batch && __ldg(kp.cum + i) == i && __ldg(kp.cum + i + 1) == i + 1) {
+    seq = i;
+  } else {
+    seq = q8_seq(kp.cum, kp.batch, i);
+    if (seq < 0) return 0;
+    past = __ldg(kp.past + seq), first = __ldg(kp.cum + seq);
+  }
+  const int pos = past + (i - first);
   return pos < 0 || pos >= (int64_t)kp.maxb * kp.bs || (kp.rot && pos >= kp.max_seq) ? 0 : pos + 1;
 }
 
@@ -177,25 +184,43 @@ __global__ void paged_q8_reset_kernel(int* counters, int n) {
   for (int t = threadIdx.x; t < n; t += blockDim.x) counters[t] = 0;
 }
 
+// 16 consecutive elements at a 16-byte aligned address
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, float (&x)[16]) {
+  uint4 w[sizeof(T)];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T); ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  const T* h = reinterpret_cast<const T*>(w);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = to_f<T>(h[e]);
+}
+
+// Pair p (dims 2p, 2p + 1) of head h in a warp's [kHeads][D] merge buffer: the 16 lanes that store at
+// once (4 g x 4 c) land on different 8-byte banks.
+template <int D>
+__device__ __forceinline__ int merge_at(int h, int p) {
+  const int c = (h >> 1) & 3;
+  const int f = D >= 128 ? ((p >> 4) & 1) | (c << 1) : D == 64 ? c : (c & 1) | ((c >> 1) << 3);
+  return h * (D / 2) + (p ^ f);
+}
+
 template <typename T, int D, int CT, int NT>
-__global__ void __launch_bounds__(kWarps * 32, (Cfg<D, NT>::kCtasPerSm))
-paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended) {
-  using C = Cfg<D, NT>;
-  constexpr bool SPLIT = std::is_same<T, float>::value;
-  constexpr int NS = SPLIT ? 2 : 1;   // fp16 terms of q and of P
-  constexpr int KW = D / 16;          // 4-byte words of a key per thread = k-steps of q.k
-  constexpr int VW = D / 32;          // 4-byte words of a value row per thread
-  constexpr int MT = D / 16;          // 16-dim tiles of the output
-  constexpr int KV = KW >= 4 ? 4 : KW;   // words of one load
-  constexpr int VV = VW >= 4 ? 4 : VW;
+__global__ void __launch_bounds__(kThreads, (Cfg<T, D, NT>::kCtasPerSm))
+paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
+  using C = Cfg<T, D, NT>;
+  constexpr int NQ = C::kNQ, NP = C::kNP, S = C::kStages, U = C::kUnit;
+  constexpr int KW = D / 16;  // 4-byte words of a key per thread = k-steps of q.k
+  constexpr int VW = D / 32;  // 4-byte words of a value row per thread
+  constexpr int MT = D / 16;  // 16-dim tiles of the output
+  constexpr int KV = KW >= 4 ? 4 : KW, VV = VW >= 4 ? 4 : VW;  // words of one load
   extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ long long plan_s[3];
-  __shared__ int scan_s[kWarps], plan_i[3], flag_s;
+  __shared__ long long plan_s;
+  __shared__ int scan_s[kWarps], plan_i, flag_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  const uint32_t sbase = smem_u32(sm);
-  const uint32_t ring = sbase + warp * C::kStages * C::kStageBytes;
-  Meta* meta = reinterpret_cast<Meta*>(sm + C::kMeta) + warp * C::kStages;
-  float* mls = reinterpret_cast<float*>(sm + C::kMl);
+  const uint32_t ring = smem_u32(sm) + warp * S * C::kStageBytes;
+  float2* mls = reinterpret_cast<float2*>(sm + C::kMl);
+  float* qscale = reinterpret_cast<float*>(sm + C::kScale);
+  float2* misc = reinterpret_cast<float2*>(sm + C::kMisc);
   const int HC = kp.HK * hchunks;
   bool waited = false;
   if (appended) {  // the launch before this one wrote rows that are read here
@@ -205,36 +230,36 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended) {
 
   // ---- this CTA's run [w0, w1) of the unit list, and the row that w0 lies in
   long long total = 0;
-  for (int i0 = 0; i0 < kp.ntok; i0 += kWarps * 32) {
-    int seq, i = i0 + tid, n = row_keys(kp, i, seq);
+  int seq0, n0 = row_keys(kp, tid, seq0);
+  for (int i0 = 0; i0 < kp.ntok; i0 += kThreads) {
+    const int i = i0 + tid, n = i0 ? row_keys(kp, i, seq0) : n0;
     if (i < kp.ntok && n == 0 && i % (int)gridDim.x == (int)blockIdx.x) {
+      if (!waited) pdl_wait();  // an earlier launch may still use `out`
       T* o = static_cast<T*>(kp.out) + (size_t)i * kp.H * D;
-      // (no launch before this one reads `out` unless it already completed or is waited for here)
-      if (!waited) pdl_wait();
       for (int e = 0; e < kp.H * D; ++e) o[e] = from_f<T>(0.f);
       report_device_error(kp.err, kErrPagedQ8, i);
     }
-    int s = (n + kUnit - 1) / kUnit;
-    s = __reduce_add_sync(0xffffffffu, s);
+    const int s = __reduce_add_sync(0xffffffffu, (n + U - 1) / U);
     if (lane == 0) scan_s[warp] = s;
     __syncthreads();
     for (int w = 0; w < kWarps; ++w) total += scan_s[w];
     __syncthreads();
   }
   const long long W = total * HC;
-  const long long ctas = max(1ll, min((long long)gridDim.x, (W + kWarps - 1) / kWarps));
+  const int ctas = (int)max(1ll, min((long long)gridDim.x, (W + kWarps - 1) / kWarps));
   const int cta = blockIdx.x;
   if (W == 0 || cta >= ctas) {
     if (!waited) pdl_wait();
     pdl_trigger();
     return;
   }
-  const long long w0 = W * cta / ctas, w1 = W * (cta + 1) / ctas;
+  const long long w0 = W * cta / ctas;
+  const int run = (int)(W * (cta + 1) / ctas - w0);
   {
     long long base = 0;
-    for (int i0 = 0; i0 < kp.ntok; i0 += kWarps * 32) {
-      int seq, i = i0 + tid, n = row_keys(kp, i, seq);
-      const int nu = (n + kUnit - 1) / kUnit;
+    for (int i0 = 0; i0 < kp.ntok; i0 += kThreads) {
+      const int i = i0 + tid, n = i0 ? row_keys(kp, i, seq0) : n0;
+      const int nu = (n + U - 1) / U;
       int inc = nu;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -243,24 +268,17 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended) {
       }
       if (lane == 31) scan_s[warp] = inc;
       __syncthreads();
-      long long pre = base;
-      int all = 0;
+      long long pre = base + inc - nu;
       for (int w = 0; w < kWarps; ++w) {
         if (w < warp) pre += scan_s[w];
-        all += scan_s[w];
+        base += scan_s[w];
       }
-      pre += inc - nu;
-      if (nu && pre * HC <= w0 && w0 < (pre + nu) * HC) {
-        plan_i[0] = i;
-        plan_s[0] = pre * HC;
-      }
-      base += all;
-      const bool found = base * HC > w0;
+      if (nu && pre * HC <= w0 && w0 < (pre + nu) * HC) plan_i = i, plan_s = pre * HC;
       __syncthreads();
-      if (found) break;
+      if (base * HC > w0) break;
     }
   }
-  // a position in the unit list: unit u of head chunk hc of row `row`
+  // a position in the unit list: unit u of head chunk hc of row `row`, which has nu units (n keys)
   struct Pos {
     int row, seq, n, nu, hc, u;
   };
@@ -273,58 +291,77 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended) {
           ++p.row;
           p.n = row_keys(kp, p.row, p.seq);
         } while (p.n == 0 && p.row < kp.ntok);
-        p.nu = (p.n + kUnit - 1) / kUnit;
-        if (p.row >= kp.ntok) {  // past the end: nothing is issued from here
-          p.nu = 0x7fffffff;
-        }
+        p.nu = p.row < kp.ntok ? (p.n + U - 1) / U : 0x7fffffff;  // (past the last row: nothing more is issued)
       }
     }
   };
   Pos at;  // the segment in work
-  at.row = plan_i[0];
+  at.row = plan_i;
   at.n = row_keys(kp, at.row, at.seq);
-  at.nu = (at.n + kUnit - 1) / kUnit;
+  at.nu = (at.n + U - 1) / U;
   {
-    const long long off = w0 - plan_s[0];
+    const long long off = w0 - plan_s;
     at.hc = (int)(off / at.nu);
     at.u = (int)(off % at.nu);
   }
 
-  // ---- the warp's stream: units x = warp, warp + 4, ... of the run
+  // ---- the warp's stream: units warp, warp + 4, ... of the run, S - 1 ahead of their use
   Pos is = at;
   is.u += warp;
   settle(is);
-  long long ix = warp;             // of the next unit to issue
-  const long long run = w1 - w0;
-  auto lookup = [&]() -> int {     // page row of key `lane` of the next unit, or -1
+  int ix = warp;  // next unit to issue, within the run
+  // whole units lie in one page (16-row aligned): one lookup a unit, else one a key
+  const bool paged = kp.bs % U == 0 && (vec & 2);
+  auto lookup = [&]() -> int {
     if (ix >= run) return -1;
-    const int key = is.u * kUnit + lane;
-    return key < is.n ? q8_row(kp.bt, kp.maxb, kp.nblocks, kp.bs, kp.HK, is.seq, is.hc / hchunks, key) : -1;
+    const int key = is.u * U + (paged ? 0 : lane);
+    return key < is.n && (paged || lane < U)
+               ? q8_row(kp.bt, kp.maxb, kp.nblocks, kp.bs, kp.HK, is.seq, hchunks == 1 ? is.hc : is.hc / hchunks, key)
+               : -1;
   };
   int next_row = lookup();
   bool bad = false;
+  uint32_t valid_q[S - 1];  // of the units in flight, the oldest first
+  constexpr int CH = D / 16, PER = U * CH / 32;  // 16-byte chunks of a row; of a unit's K per lane
   auto issue = [&](int stage) {
+    uint32_t valid = 0;
     if (ix < run) {
-      const int row = next_row, key = is.u * kUnit + lane;
-      bad |= row < 0 && key < is.n;
+      const int row = next_row, left = is.n - is.u * U;  // keys from this unit's first on
       const uint32_t dst = ring + stage * C::kStageBytes;
-      constexpr int CH = D / 16;  // chunks of a row
+      const uint32_t inside = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+      if (paged) {
+        bad |= row < 0;
+        if (row >= 0) {
+          valid = inside;
+          const size_t o = (size_t)row * D + lane * 16;
+          const uint8_t *ks = kp.kc + o, *vs = kp.vc + o;
 #pragma unroll
-      for (int t = 0; t < CH; ++t) {
-        const int idx = t * 32 + lane, r = idx / CH, ch = idx % CH;
-        const int src = __shfl_sync(0xffffffffu, row, r);
-        const size_t o = (size_t)(src < 0 ? 0 : src) * D + ch * 16;
-        const uint32_t d = dst + swz<D>(r, ch);
-        cp16(d, kp.kc + o, src >= 0);
-        cp16(d + C::kData, kp.vc + o, src >= 0);
-      }
-      cp4(dst + 2 * C::kData + lane * 4, kp.kscale + (row < 0 ? 0 : row), row >= 0);
-      cp4(dst + 2 * C::kData + kUnit * 4 + lane * 4, kp.vscale + (row < 0 ? 0 : row), row >= 0);
-      const uint32_t valid = __ballot_sync(0xffffffffu, row >= 0);
-      if (lane == 0) {
-        Meta m;
-        m.row = is.row, m.hc = is.hc, m.u = is.u, m.n = is.n, m.valid = valid;
-        meta[stage] = m;
+          for (int t = 0; t < PER; ++t) {
+            const uint32_t d = dst + swz<D>((t * 32 + lane) / CH, (t * 32 + lane) % CH);
+            cp16(d, ks + t * 512);
+            cp16(d + C::kData, vs + t * 512);
+          }
+          if (lane < U / 4) cp16(dst + 2 * C::kData + lane * 16, kp.kscale + row + lane * 4);
+          else if (lane < U / 2) cp16(dst + 2 * C::kData + lane * 16, kp.vscale + row + (lane - U / 4) * 4);
+        }
+      } else {
+        bad |= row < 0 && lane < U && lane < left;
+        valid = __ballot_sync(0xffffffffu, row >= 0);
+#pragma unroll
+        for (int t = 0; t < PER; ++t) {
+          const int r = (t * 32 + lane) / CH, ch = (t * 32 + lane) % CH;
+          const int src = __shfl_sync(0xffffffffu, row, r);
+          if (src >= 0) {
+            const size_t o = (size_t)src * D + ch * 16;
+            const uint32_t d = dst + swz<D>(r, ch);
+            cp16(d, kp.kc + o);
+            cp16(d + C::kData, kp.vc + o);
+          }
+        }
+        if (row >= 0) {
+          cp4(dst + 2 * C::kData + lane * 4, kp.kscale + row);
+          cp4(dst + 2 * C::kData + U * 4 + lane * 4, kp.vscale + row);
+        }
       }
       ix += kWarps;
       is.u += kWarps;
@@ -332,50 +369,76 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended) {
       next_row = lookup();
     }
     cp_commit();
+#pragma unroll
+    for (int i = 0; i + 1 < S - 1; ++i) valid_q[i] = valid_q[i + 1];
+    valid_q[S - 2] = valid;
   };
 #pragma unroll
-  for (int s = 0; s < C::kStages - 1; ++s) issue(s);
+  for (int i = 0; i < S - 1; ++i) valid_q[i] = 0;
+#pragma unroll 1
+  for (int i = 0; i < S - 1; ++i) issue(i);
 
   int stage = 0;
-  long long x = 0;  // first unit of the segment, within the run
-  long long mine = warp;  // the warp's next unit
+  int x = 0;        // first unit of the segment, within the run
+  int mine = warp;  // the warp's next unit
   while (x < run) {
-    const int nseg = (int)min((long long)(at.nu - at.u), run - x);  // units of this segment
-    const int kvh = at.hc / hchunks, h0 = kvh * kp.G + (at.hc % hchunks) * C::kHeads;  // first query head
-    const int heads = min(C::kHeads, kp.G - (at.hc % hchunks) * C::kHeads);
-    // q as the second operand: thread (g, c) holds head g, the dims of its key bytes
-    uint32_t qf[NS][NT][KW][2];
-    float qs[NT][2];  // per owned score column (heads 2c, 2c + 1): what turns a score into base-2 logits
+    const int nseg = min(at.nu - at.u, run - x);  // units of this segment
+    const int chunk = hchunks == 1 ? 0 : at.hc % hchunks;
+    const int h0 = (hchunks == 1 ? at.hc : at.hc / hchunks) * kp.G + chunk * C::kHeads;  // first query head
+    const int heads = min(C::kHeads, kp.G - chunk * C::kHeads);
+    // ---- q as the second operand, in shared memory: 16 dims of a head per thread, D / 16 threads a head
+    constexpr uint32_t kQLanes = C::kHeads * CH >= 32 ? 0xffffffffu : 0xffffu;  // (16 or a multiple of 32 threads)
+    if (tid < C::kHeads * CH) {
+      const int h = tid / CH, ch = tid % CH, d0 = ch * 16, pos = at.n - 1;
+      float q[16];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int hq = nt * 8 + g;
-      const T* qrow = static_cast<const T*>(kp.q) + (size_t)at.row * kp.qs + (size_t)(h0 + hq) * D;
-      float qv[KW * 4];
-      float amax = 0.f;
+      for (int e = 0; e < 16; ++e) q[e] = 0.f;
+      if (h < heads) {
+        const T* row = static_cast<const T*>(kp.q) + (size_t)at.row * kp.qs + (size_t)(h0 + h) * D;
+        if (vec & 1) {  // aligned rows, halves of whole 16-dim chunks
+          load16<T>(row + d0, q);
+          if (kp.rot && d0 < 2 * kp.half) {
+            const bool first = d0 < kp.half;
+            const int i0 = first ? d0 : d0 - kp.half;
+            float y[16], cs[16], sn[16];
+            load16<T>(row + (first ? d0 + kp.half : i0), y);
+            load16<T>(static_cast<const T*>(kp.cos_c) + (size_t)pos * kp.half + i0, cs);
+            load16<T>(static_cast<const T*>(kp.sin_c) + (size_t)pos * kp.half + i0, sn);
 #pragma unroll
-      for (int w = 0; w < KW; ++w)
+            for (int e = 0; e < 16; ++e)
+              q[e] = first ? __fsub_rn(__fmul_rn(q[e], cs[e]), __fmul_rn(y[e], sn[e]))
+                           : __fadd_rn(__fmul_rn(q[e], cs[e]), __fmul_rn(y[e], sn[e]));
+          }
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          qv[w * 4 + e] = hq < heads ? q_at<T>(qrow, kbyte<D>(c, w) + e, kp, at.n - 1) : 0.f;
-          amax = fmaxf(amax, fabsf(qv[w * 4 + e]));
+          for (int e = 0; e < 16; ++e) q[e] = q_at<T>(row, d0 + e, kp, pos);
         }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const int ex = min(max((int)(__float_as_uint(amax) >> 23), 1), 253);  // biased exponent
-      const float down = __uint_as_float((uint32_t)(254 - ex) << 23), up = __uint_as_float((uint32_t)ex << 23);
+      }
+      uint32_t amax = 0;
 #pragma unroll
-      for (int w = 0; w < KW; ++w)
+      for (int e = 0; e < 16; ++e) amax = max(amax, __float_as_uint(q[e]) & 0x7fffffffu);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float a = qv[w * 4 + 2 * e] * down, b = qv[w * 4 + 2 * e + 1] * down;
-          const __half2 hi = __floats2half2_rn(a, b);
-          qf[0][nt][w][e] = *reinterpret_cast<const uint32_t*>(&hi);
-          if constexpr (SPLIT) qf[1][nt][w][e] = half2_bits(a - __low2float(hi), b - __high2float(hi));
+      for (int o = CH / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(kQLanes, amax, o));
+      const int ex = min(max((int)(amax >> 23), 1), 253);  // biased exponent
+      const float down = __uint_as_float((uint32_t)(254 - ex) << 23);
+      if (ch == 0)
+        qscale[h] = __uint_as_float((uint32_t)ex << 23) * kp.scale * (CT == kE4M3 ? 256.f : 1.f) * 1.4426950408889634f;
+#pragma unroll
+      for (int w4 = 0; w4 < 4; ++w4) {  // 4 dims: word w of thread (h % 8, qc)
+        const int qc = D >= 128 ? (ch & 7) >> 1 : D == 64 ? ch : 2 * ch + (w4 >> 1);
+        const int w = D >= 128 ? (ch >> 3) * 8 + (ch & 1) * 4 + w4 : D == 64 ? w4 : w4 & 1;
+        const float a0 = q[w4 * 4] * down, a1 = q[w4 * 4 + 1] * down, a2 = q[w4 * 4 + 2] * down, a3 = q[w4 * 4 + 3] * down;
+        const __half2 p0 = __floats2half2_rn(a0, a1), p1 = __floats2half2_rn(a2, a3);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(sm + C::kQ) +
+                        (size_t)(((h >> 3) * KW + w) * 32 + (h & 7) * 4 + qc) * (2 * NQ);
+        dst[0] = *reinterpret_cast<const uint32_t*>(&p0), dst[1] = *reinterpret_cast<const uint32_t*>(&p1);
+        if constexpr (NQ == 2) {
+          dst[2] = half2_bits(a0 - __low2float(p0), a1 - __high2float(p0));
+          dst[3] = half2_bits(a2 - __low2float(p1), a3 - __high2float(p1));
         }
-      const float f = up * kp.scale * (CT == kE4M3 ? 256.f : 1.f) * 1.4426950408889634f;
-      qs[nt][0] = __shfl_sync(0xffffffffu, f, 8 * c);
-      qs[nt][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
+      }
     }
+    __syncthreads();  // q is there; the merge buffers of the segment before are free
 
     float o[MT][NT][4], m[NT][2], l[NT][2];
     int E = kLift + 1;  // biased exponent that P vs is relative to
@@ -386,24 +449,24 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended) {
       for (int t = 0; t < MT; ++t) o[t][nt][0] = o[t][nt][1] = o[t][nt][2] = o[t][nt][3] = 0.f;
     }
 
+#pragma unroll 1
     for (; mine < x + nseg; mine += kWarps) {
-      cp_wait<C::kStages - 2>();
+      cp_wait<S - 2>();
       __syncwarp();
-      const int ahead = stage == 0 ? C::kStages - 1 : stage - 1;  // the buffer that was consumed last
-      issue(ahead);
+      const uint32_t valid_u = valid_q[0];
+      issue(stage == 0 ? S - 1 : stage - 1);  // into the buffer that was consumed last
       const uint32_t buf = ring + stage * C::kStageBytes;
-      const uint32_t valid = meta[stage].valid;
-      const uint32_t sks = buf + 2 * C::kData, svs = sks + kUnit * 4;
-      // S^T: two 16-key tiles
-      float s[2][NT][4];
+#pragma unroll 1
+      for (int kt = 0; kt < NT; ++kt) {  // 16 keys
+        const uint32_t valid = valid_u >> (kt * 16);
+        const uint32_t sks = buf + 2 * C::kData + kt * 64, svs = sks + U * 4;
+        float s[NT][4];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
+        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[kt][nt][0] = s[kt][nt][1] = s[kt][nt][2] = s[kt][nt][3] = 0.f;
-#pragma unroll
-        for (int w0_ = 0; w0_ < KW; w0_ += KV) {
+        for (int wb = 0; wb < KW; wb += KV) {
           uint32_t ka[KV], kb[KV];
-          const int r0 = kt * 16 + g, byte = kbyte<D>(c, w0_);
+          const int r0 = kt * 16 + g, byte = kbyte<D>(c, wb);
           lds<KV * 4>(buf + swz<D>(r0, byte >> 4) + (byte & 15), ka);
           lds<KV * 4>(buf + swz<D>(r0 + 8, byte >> 4) + (byte & 15), kb);
 #pragma unroll
@@ -412,91 +475,76 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended) {
             widen<CT>(ka[w], a[0], a[2]);
             widen<CT>(kb[w], a[1], a[3]);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+              uint32_t b[2 * NQ];
+              lds<8 * NQ>(smem_u32(sm) + C::kQ + ((nt * KW + wb + w) * 32 + lane) * (8 * NQ), b);
 #pragma unroll
-              for (int t = 0; t < NS; ++t) mma(s[kt][nt], a, qf[t][nt][w0_ + w][0], qf[t][nt][w0_ + w][1]);
+              for (int t = 0; t < NQ; ++t) mma(s[nt], a, b[2 * t], b[2 * t + 1]);
+            }
           }
         }
-      }
-      // scores in base 2; keys g and g + 8 of each tile
-      float vsk[2][2];
-      float mx[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mx[nt][0] = m[nt][0], mx[nt][1] = m[nt][1];
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+        // scores in base 2: key g (r = 0) and g + 8 (r = 1), heads 2c and 2c + 1
+        float vs[2];
+        bool move = false;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int key = kt * 16 + r * 8 + g;
-          const float ks = lds_f(sks + key * 4);
-          const bool on = (valid >> key) & 1u;
-          vsk[kt][r] = lds_f(svs + key * 4);
+          const bool on = (valid >> (g + r * 8)) & 1u;
+          const float ks = lds_f(sks + (g + r * 8) * 4);
+          vs[r] = on ? lds_f(svs + (g + r * 8) * 4) : 0.f;
+          move |= __float_as_uint(vs[r]) >= (uint32_t)(E + 1) << 23;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float v = on ? s[kt][nt][r * 2 + h] * (ks * qs[nt][h]) : -INFINITY;
-              s[kt][nt][r * 2 + h] = v;
-              mx[nt][h] = fmaxf(mx[nt][h], v);
+              const float v = on ? s[nt][r * 2 + h] * (ks * lds_f(smem_u32(qscale) + (nt * 8 + 2 * c + h) * 4)) : -INFINITY;
+              s[nt][r * 2 + h] = v;
+              move |= v > m[nt][h] + kSlack;
             }
         }
-      bool moved = false;
+        if (__any_sync(0xffffffffu, move)) {  // a larger score, or a larger value scale: rescale what there is
+          const int eu = (int)(__reduce_max_sync(0xffffffffu, max(__float_as_uint(vs[0]), __float_as_uint(vs[1]))) >> 23);
+          const int En = min(max(E, eu), 253);
+          const float back = __uint_as_float((uint32_t)max(127 + E - En, 0) << 23);
+          E = En;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2; ++h) {
+              float mx = fmaxf(m[nt][h], fmaxf(s[nt][h], s[nt][2 + h]));
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) mx[nt][h] = fmaxf(mx[nt][h], __shfl_xor_sync(0xffffffffu, mx[nt][h], d));
-          moved |= mx[nt][h] > m[nt][h];
+              for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+              const float a = m[nt][h] == -INFINITY ? 0.f : ex2(m[nt][h] - mx);
+              m[nt][h] = mx;
+              l[nt][h] *= a;
+#pragma unroll
+              for (int t = 0; t < MT; ++t) o[t][nt][h] *= a * back, o[t][nt][2 + h] *= a * back;
+            }
         }
-      // the running power of two of the value scales
-      const int eu = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(lds_f(svs + lane * 4))) >> 23);
-      const int En = min(max(E, eu), 253);
-      if (En != E || __any_sync(0xffffffffu, moved)) {
-        const float back = __uint_as_float((uint32_t)max(127 + E - En, 0) << 23);
+        const float down = __uint_as_float((uint32_t)(254 + kLift - E) << 23);
+        // P^T as the second operand
+        uint32_t pf[NP][NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float a = m[nt][h] == -INFINITY ? 0.f : ex2(m[nt][h] - mx[nt][h]);
-            l[nt][h] *= a;
-            m[nt][h] = mx[nt][h];
-#pragma unroll
-            for (int t = 0; t < MT; ++t) o[t][nt][h] *= a * back, o[t][nt][2 + h] *= a * back;
-          }
-        E = En;
-      }
-      const float down = __uint_as_float((uint32_t)(254 + kLift - E) << 23);  // 2^(127 + kLift - E)
-      // P^T into the second operand
-      uint32_t pf[NS][2][NT][2];
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float vs = vsk[kt][r] * down;
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float p[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float v = s[kt][nt][r * 2 + h];
+              const float v = s[nt][r * 2 + h];
               p[h] = v == -INFINITY ? 0.f : ex2(v - m[nt][h]);
               l[nt][h] += p[h];
-              p[h] *= vs;
+              p[h] *= vs[r] * down;
             }
             const __half2 hi = __floats2half2_rn(p[0], p[1]);
-            pf[0][kt][nt][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
-            if constexpr (SPLIT)
-              pf[1][kt][nt][r] = transpose8x8(half2_bits(p[0] - __low2float(hi), p[1] - __high2float(hi)));
+            pf[0][nt][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
+            if constexpr (NP == 2)
+              pf[1][nt][r] = transpose8x8(half2_bits(p[0] - __low2float(hi), p[1] - __high2float(hi)));
           }
-        }
-      // O^T += V^T P^T
+        // O^T += V^T P^T
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int w0_ = 0; w0_ < VW; w0_ += VV) {
+        for (int wb = 0; wb < VW; wb += VV) {
           uint32_t v[4][VV];  // value rows 2c, 2c + 1, 2c + 8, 2c + 9
-          const int byte = vbyte<D>(g, w0_);
+          const int byte = vbyte<D>(g, wb);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int key = kt * 16 + 2 * c + (r & 1) + (r >> 1) * 8;
@@ -504,14 +552,11 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended) {
           }
 #pragma unroll
           for (int w = 0; w < VV; ++w) {
-            // codes of two keys side by side, dim by dim
-            uint32_t d01[2], d23[2], d[2][4];
-            d01[0] = prmt(v[0][w], v[1][w], 0x5140), d23[0] = prmt(v[0][w], v[1][w], 0x7362);
-            d01[1] = prmt(v[2][w], v[3][w], 0x5140), d23[1] = prmt(v[2][w], v[3][w], 0x7362);
+            uint32_t d[2][4];  // two keys side by side, dim by dim
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              widen<CT>(d01[r], d[r][0], d[r][1]);
-              widen<CT>(d23[r], d[r][2], d[r][3]);
+              widen<CT>(prmt(v[2 * r][w], v[2 * r + 1][w], 0x5140), d[r][0], d[r][1]);
+              widen<CT>(prmt(v[2 * r][w], v[2 * r + 1][w], 0x7362), d[r][2], d[r][3]);
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -519,145 +564,106 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended) {
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int u = 0; u < NS; ++u) mma(o[(w0_ + w) * 2 + t][nt], a, pf[u][kt][nt][0], pf[u][kt][nt][1]);
+                for (int u = 0; u < NP; ++u) mma(o[(wb + w) * 2 + t][nt], a, pf[u][nt][0], pf[u][nt][1]);
             }
           }
         }
+      }
       __syncwarp();
-      stage = stage + 1 == C::kStages ? 0 : stage + 1;
+      stage = stage + 1 == S ? 0 : stage + 1;
     }
 
-    // ---- the segment's end: join the warps
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], d);
-    if (g == 0)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int hd = nt * 8 + 2 * c + h;
-          mls[(warp * C::kHeads + hd) * 2] = m[nt][h];
-          mls[(warp * C::kHeads + hd) * 2 + 1] = l[nt][h];
-        }
-    __syncthreads();
-    float mt_[NT][2], lt[NT][2];
+    // ---- the segment's end: each warp leaves (m, l, o) in its one buffer that no copy is in flight to
+    const int freeb = stage == 0 ? S - 1 : stage - 1;
     {
-      const float unscale = __uint_as_float((uint32_t)min(E, 253) << 23) * (CT == kE4M3 ? 0x1p-6f : 0x1p-14f);
-      static_assert(kLift == 14, "the power above");
+      float2* mg = reinterpret_cast<float2*>(sm + (warp * S + freeb) * C::kStageBytes);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], d);
           const int hd = nt * 8 + 2 * c + h;
-          float mm = -INFINITY, ll = 0.f;
+          if (g == 0) mls[warp * C::kHeads + hd] = make_float2(m[nt][h], l[nt][h]);
+          if (hd < heads)
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, mls[(w * C::kHeads + hd) * 2]);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float lw = mls[(w * C::kHeads + hd) * 2 + 1];
-            if (lw != 0.f) ll += lw * ex2(mls[(w * C::kHeads + hd) * 2] - mm);  // (a NaN stays one)
-          }
-          mt_[nt][h] = mm, lt[nt][h] = ll;
-          const float f = l[nt][h] == 0.f ? 0.f : ex2(m[nt][h] - mm) * unscale;  // 0: the warp saw no key, o = 0
-#pragma unroll
-          for (int t = 0; t < MT; ++t) o[t][nt][h] *= f, o[t][nt][2 + h] *= f;
+            for (int t = 0; t < MT; ++t)
+              mg[merge_at<D>(hd, (vbyte<D>(g, t >> 1) >> 1) + (t & 1))] = make_float2(o[t][nt][h], o[t][nt][2 + h]);
         }
-    }
-    // warps 2, 3 hand theirs to 0, 1, then 1 to 0 (always the same order of additions)
-    float* mg = reinterpret_cast<float*>(sm + C::kMerge);
-    constexpr int MS = D + 4;
-    auto put = [&](int slot) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int t = 0; t < MT; ++t)
-            *reinterpret_cast<float2*>(mg + (slot * C::kHeads + nt * 8 + 2 * c + h) * MS + vbyte<D>(g, t >> 1) + (t & 1) * 2) =
-                make_float2(o[t][nt][h], o[t][nt][2 + h]);
-    };
-    auto add = [&](int slot) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            const float2 v = *reinterpret_cast<const float2*>(
-                mg + (slot * C::kHeads + nt * 8 + 2 * c + h) * MS + vbyte<D>(g, t >> 1) + (t & 1) * 2);
-            o[t][nt][h] += v.x, o[t][nt][2 + h] += v.y;
-          }
-    };
-    if (warp >= 2) put(warp - 2);
-    __syncthreads();
-    if (warp < 2) add(warp);
-    __syncthreads();
-    if (warp == 1) put(0);
-    __syncthreads();
-    if (warp == 0) {
-      add(0);
-      put(1);
-      if (g == 0)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int hd = nt * 8 + 2 * c + h;
-            mls[hd * 2] = mt_[nt][h];  // (every warp has read the others' by now)
-            mls[hd * 2 + 1] = lt[nt][h];
-          }
+      static_assert(kLift == 6, "the powers below");
+      if (lane == 0)
+        misc[warp] = make_float2(__uint_as_float((uint32_t)E << 23) * (CT == kE4M3 ? 4.f : 0x1p-6f), __int_as_float(freeb));
     }
     __syncthreads();
-    const float* res = mg + C::kHeads * MS;
     const bool whole = nseg == at.nu;
     if (!waited) {  // before anything is written
       pdl_wait();
       waited = true;
     }
     T* out = static_cast<T*>(kp.out) + (size_t)at.row * kp.H * D + (size_t)h0 * D;
-    if (whole) {
-      for (int e = tid; e < heads * D; e += kWarps * 32) {
-        const int hd = e / D;
-        const float ll = mls[hd * 2 + 1];
-        out[e] = from_f<T>(ll == 0.f ? 0.f : res[hd * MS + e % D] / ll);
+    const int slot = 2 * cta + (at.u > 0 ? 0 : 1);
+    float* part = kp.part + (size_t)slot * C::kHeads * (D + 2);
+    for (int e = tid; e < heads * (D / 2); e += kThreads) {
+      const int hd = e / (D / 2), p = e % (D / 2);
+      float2 ml[kWarps], acc = make_float2(0.f, 0.f);
+      float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        ml[w] = mls[w * C::kHeads + hd];
+        mm = fmaxf(mm, ml[w].x);
       }
-    } else {
-      const int slot = 2 * cta + (at.u > 0 ? 0 : 1);
-      float* part = kp.part + (size_t)slot * C::kHeads * (D + 2);
-      for (int e = tid; e < heads * D; e += kWarps * 32) part[(e / D) * (D + 2) + e % D] = res[(e / D) * MS + e % D];
-      if (tid < 2 * heads) part[(tid >> 1) * (D + 2) + D + (tid & 1)] = mls[tid];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (ml[w].y == 0.f) continue;  // the warp saw no key of this segment (a NaN is not 0)
+        const float2 us = misc[w];
+        const float f = ex2(ml[w].x - mm);
+        const float2 v = reinterpret_cast<const float2*>(sm + (w * S + __float_as_int(us.y)) * C::kStageBytes)[merge_at<D>(hd, p)];
+        ll += ml[w].y * f;
+        acc.x += v.x * (f * us.x), acc.y += v.y * (f * us.x);
+      }
+      if (whole) {
+        const float r = ll == 0.f ? 0.f : __frcp_rn(ll);
+        out[hd * D + 2 * p] = from_f<T>(acc.x * r), out[hd * D + 2 * p + 1] = from_f<T>(acc.y * r);
+      } else {
+        *reinterpret_cast<float2*>(part + hd * D + 2 * p) = acc;
+        if (p == 0) *reinterpret_cast<float2*>(part + C::kHeads * D + hd * 2) = make_float2(mm, ll);
+      }
+    }
+    if (!whole) {
       __threadfence();
       __syncthreads();
-      // the runs that hold units of this (row, head chunk)
+      // the runs that hold units of this (row, head chunk); in the first of them it is the last segment
       const long long a = w0 + x - at.u, z = a + at.nu;
       const int kf = (int)(((a + 1) * ctas - 1) / W), kl = (int)((z * ctas - 1) / W);
       if (tid == 0) flag_s = atomicAdd(kp.counters + kf, 1) == kl - kf;
       __syncthreads();
-      if (flag_s) {  // the last to arrive joins the parts
+      if (flag_s) {  // the last to arrive joins the parts, in the order of the keys
         __threadfence();
-        for (int e = tid; e < heads * D; e += kWarps * 32) {
-          const int hd = e / D;
-          float mm = -INFINITY, ll = 0.f, acc = 0.f;
-          for (int k = kf; k <= kl; ++k) {
-            const long long k0 = W * k / ctas;
-            const float* pp = kp.part + ((size_t)(2 * k + (k0 > a ? 0 : 1)) * C::kHeads + hd) * (D + 2);
-            const float mk = __ldcg(pp + D), lk = __ldcg(pp + D + 1), ok = __ldcg(pp + e % D);
-            if (lk == 0.f) continue;
-            const float mn = fmaxf(mm, mk);
-            const float fa = mm == -INFINITY ? 0.f : ex2(mm - mn), fb = ex2(mk - mn);
-            ll = ll * fa + lk * fb;
-            acc = acc * fa + ok * fb;
-            mm = mn;
+        const size_t step = (size_t)2 * C::kHeads * (D + 2);  // from one run's first part to the next one's
+        const float* first = kp.part + (size_t)(2 * kf + 1) * C::kHeads * (D + 2);
+        const float* rest = kp.part + (size_t)(2 * kf) * C::kHeads * (D + 2);
+        for (int e = tid; e < heads * (D / 4); e += kThreads) {
+          const int hd = e / (D / 4), d = (e % (D / 4)) * 4;
+          float mm = __ldcg(first + C::kHeads * D + hd * 2);
+#pragma unroll 8
+          for (int k = 1; k <= kl - kf; ++k) mm = fmaxf(mm, __ldcg(rest + k * step + C::kHeads * D + hd * 2));
+          float ll = 0.f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int k = 0; k <= kl - kf; ++k) {
+            const float* pp = k ? rest + k * step : first;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(pp + C::kHeads * D + hd * 2));
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(pp + hd * D + d));
+            const float f = ml.y == 0.f ? 0.f : ex2(ml.x - mm);
+            ll += ml.y * f;
+            acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
           }
-          out[e] = from_f<T>(ll == 0.f ? 0.f : acc / ll);
+          const float r = ll == 0.f ? 0.f : __frcp_rn(ll);
+          T* q = out + hd * D + d;
+          q[0] = from_f<T>(acc.x * r), q[1] = from_f<T>(acc.y * r), q[2] = from_f<T>(acc.z * r), q[3] = from_f<T>(acc.w * r);
         }
       }
     }
-    __syncthreads();  // the merge buffers and mls are free again
     x += nseg;
     at.u += nseg;
     if (x < run) settle(at);
@@ -669,14 +675,19 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended) {
 
 template <typename T, int D, int CT, int NT>
 cudaError_t launch_t(const PagedQ8& a, bool appended, cudaStream_t st) {
-  using C = Cfg<D, NT>;
+  using C = Cfg<T, D, NT>;
   auto kern = paged_q8_attn_kernel<T, D, CT, NT>;
   if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kTotal)) return e;
-  if (!appended)
-    if (cudaError_t e = launch_k(paged_q8_reset_kernel, dim3(1), dim3(256), 0, st, a.counters, a.ctas)) return e;
-  const int hchunks = (a.G + C::kHeads - 1) / C::kHeads;
   const int grid = std::min(a.ctas, num_sms() * C::kCtasPerSm);
-  return launch_k(kern, dim3((unsigned)grid), dim3(kWarps * 32), C::kTotal, st, a, hchunks, appended ? 1 : 0);
+  if (!appended)
+    if (cudaError_t e = launch_k(paged_q8_reset_kernel, dim3(1), dim3(256), 0, st, a.counters, grid)) return e;
+  const int hchunks = (a.G + C::kHeads - 1) / C::kHeads;
+  auto al = [](const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && bytes % 16 == 0; };
+  const int es = (int)sizeof(T);
+  int vec = al(a.q, a.qs * es) &&
+            (!a.rot || (!a.inter && a.half % 16 == 0 && al(a.cos_c, (int64_t)a.half * es) && al(a.sin_c, 0)));
+  if (al(a.kscale, 0) && al(a.vscale, 0)) vec |= 2;
+  return launch_k(kern, dim3((unsigned)grid), dim3(kThreads), C::kTotal, st, a, hchunks, appended ? 1 : 0, vec);
 }
 
 template <typename T, int D, int CT>
@@ -685,7 +696,6 @@ cudaError_t by_group(const PagedQ8& a, bool appended, cudaStream_t st) {
     if (paged_q8_heads_per_cta(D, a.G) == 16) return launch_t<T, D, CT, 2>(a, appended, st);
   return launch_t<T, D, CT, 1>(a, appended, st);
 }
-
 template <typename T, int CT>
 cudaError_t by_head(const PagedQ8& a, bool appended, cudaStream_t st) {
   switch (a.D) {
@@ -699,7 +709,7 @@ cudaError_t by_head(const PagedQ8& a, bool appended, cudaStream_t st) {
 
 }  // namespace
 
-int paged_q8_max_ctas() { return 2 * num_sms(); }
+int paged_q8_max_ctas() { return 4 * num_sms(); }
 // more than 8 query heads per kv head: 16 to a CTA (two column tiles share each widened code), except
 // at head size 256, whose output tile would not fit the registers
 int paged_q8_heads_per_cta(int D, int G) { return G > 8 && D <= 128 ? 16 : 8; }

@@ -10,7 +10,7 @@
 namespace b200ep {
 namespace {
 
-constexpr size_t kCounterBytes = 4096;  // arrival counters at the front of the workspace
+constexpr size_t kCounterBytes = 8192;  // arrival counters at the front of the workspace
 
 int check_geometry(const b200ep_paged_q8_params* p, int dtype, const char* op) {
   const std::string n = op;
