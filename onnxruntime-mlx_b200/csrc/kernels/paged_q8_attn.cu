@@ -40,9 +40,10 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kLift = 6;       // P vs is held times 2^kLift
 constexpr float kSlack = 8.f;  // a score may pass the running maximum by this much (in base 2) before it moves
 
-template <typename T, int D, int NT>
+template <typename T, int D, int CT, int NT>
 struct Cfg {
-  static constexpr int kNQ = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;  // fp16 terms of q
+  static constexpr bool kInt = CT == kI8;  // K Q^T on 8-bit integers: q as kNQ bytes; else q as kNQ fp16 terms
+  static constexpr int kNQ = kInt + (std::is_same<T, __nv_bfloat16>::value ? 1 : 2);
   static constexpr int kNP = std::is_same<T, float>::value ? 2 : 1;          // fp16 terms of P
   static constexpr int kUnit = 16 * NT;  // keys of a unit
   static constexpr int kHeads = 8 * NT;  // query heads of a CTA
@@ -51,7 +52,7 @@ struct Cfg {
   static constexpr int kData = kUnit * D;                         // K (or V) codes of a unit
   static constexpr int kStageBytes = 2 * kData + 2 * kUnit * 4;   // K, V, ks, vs; holds [kHeads][D] fp32 at a merge
   static constexpr int kQ = kWarps * kStages * kStageBytes;       // the query operand
-  static constexpr int kQBytes = kNQ * NT * (D / 16) * 32 * 8;
+  static constexpr int kQBytes = kNQ * NT * (D / 16) * 32 * (kInt ? 4 : 8);
   static constexpr int kMl = kQ + kQBytes;                        // [kWarps][kHeads] (m, l)
   static constexpr int kScale = kMl + kWarps * kHeads * 8;        // [kHeads] score factor
   static constexpr int kMisc = kScale + kHeads * 4;               // [kWarps] (output factor, buffer)
@@ -92,7 +93,7 @@ __host__ __device__ __forceinline__ constexpr int vbyte(int g, int w) {
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
-// The four codes of a word as two f16x2 (codes 0, 1 and 2, 3); e4m3 values come out times 2^-8.
+// The four codes of a word as two f16x2 (codes 0, 1 and 2, 3).
 template <int CT>
 __device__ __forceinline__ void widen(uint32_t w, uint32_t& h01, uint32_t& h23) {
   if constexpr (CT == kI8) {
@@ -103,10 +104,8 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& h01, uint32_t& h23) 
     __half2 ha = __hsub2(*reinterpret_cast<__half2*>(&a), bias), hb = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
     h01 = *reinterpret_cast<uint32_t*>(&ha), h23 = *reinterpret_cast<uint32_t*>(&hb);
   } else {
-    // sign to bit 15, exponent and mantissa to bits 13..7: the same number with fp16's bias, 2^8 lower
-    const uint32_t a = prmt(w, 0, 0x1404), b = prmt(w, 0, 0x3424);
-    h01 = ((a >> 1) & 0x3f803f80u) | (a & 0x80008000u);
-    h23 = ((b >> 1) & 0x3f803f80u) | (b & 0x80008000u);
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(h01), "=r"(h23) : "r"(w));
   }
 }
 
@@ -114,6 +113,12 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -132,11 +137,11 @@ __device__ __forceinline__ float ex2(float x) {
 template <int BYTES>
 __device__ __forceinline__ void lds(uint32_t addr, uint32_t* r) {
   if constexpr (BYTES == 16)
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
   else if constexpr (BYTES == 8)
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
   else
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(addr));
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ float lds_f(uint32_t addr) {
   float v;
@@ -205,9 +210,9 @@ __device__ __forceinline__ int merge_at(int h, int p) {
 }
 
 template <typename T, int D, int CT, int NT>
-__global__ void __launch_bounds__(kThreads, (Cfg<T, D, NT>::kCtasPerSm))
+__global__ void __launch_bounds__(kThreads, (Cfg<T, D, CT, NT>::kCtasPerSm))
 paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
-  using C = Cfg<T, D, NT>;
+  using C = Cfg<T, D, CT, NT>;
   constexpr int NQ = C::kNQ, NP = C::kNP, S = C::kStages, U = C::kUnit;
   constexpr int KW = D / 16;  // 4-byte words of a key per thread = k-steps of q.k
   constexpr int VW = D / 32;  // 4-byte words of a value row per thread
@@ -328,7 +333,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
     if (ix < run) {
       const int row = next_row, left = is.n - is.u * U;  // keys from this unit's first on
       const uint32_t dst = ring + stage * C::kStageBytes;
-      const uint32_t inside = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+      const uint32_t inside = left >= U ? (U == 32 ? 0xffffffffu : 0xffffu) : (1u << left) - 1u;
       if (paged) {
         bad |= row < 0;
         if (row >= 0) {
@@ -419,22 +424,55 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       for (int e = 0; e < 16; ++e) amax = max(amax, __float_as_uint(q[e]) & 0x7fffffffu);
 #pragma unroll
       for (int o = CH / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(kQLanes, amax, o));
-      const int ex = min(max((int)(amax >> 23), 1), 253);  // biased exponent
-      const float down = __uint_as_float((uint32_t)(254 - ex) << 23);
-      if (ch == 0)
-        qscale[h] = __uint_as_float((uint32_t)ex << 23) * kp.scale * (CT == kE4M3 ? 256.f : 1.f) * 1.4426950408889634f;
+      const float base = kp.scale * 1.4426950408889634f;
+      if constexpr (C::kInt) {
+        // q / amax as an integer of kNQ bytes, each in [-128, 127]
+        const float top = __uint_as_float(amax), M = NQ == 3 ? 127.f * 65536.f : 127.f * 256.f;
+        const float up = amax && amax < 0x7f800000u ? __fdiv_rn(M, top) : 0.f;
+        if (ch == 0)  // what the sum in units of the upper two bytes' last place stands for
+          qscale[h] = amax < 0x7f800000u ? top * base * (NQ == 3 ? 256.f / (127.f * 65536.f) : 1.f / (127.f * 256.f))
+                                         : __uint_as_float(0x7fc00000u);
 #pragma unroll
-      for (int w4 = 0; w4 < 4; ++w4) {  // 4 dims: word w of thread (h % 8, qc)
-        const int qc = D >= 128 ? (ch & 7) >> 1 : D == 64 ? ch : 2 * ch + (w4 >> 1);
-        const int w = D >= 128 ? (ch >> 3) * 8 + (ch & 1) * 4 + w4 : D == 64 ? w4 : w4 & 1;
-        const float a0 = q[w4 * 4] * down, a1 = q[w4 * 4 + 1] * down, a2 = q[w4 * 4 + 2] * down, a3 = q[w4 * 4 + 3] * down;
-        const __half2 p0 = __floats2half2_rn(a0, a1), p1 = __floats2half2_rn(a2, a3);
-        uint32_t* dst = reinterpret_cast<uint32_t*>(sm + C::kQ) +
-                        (size_t)(((h >> 3) * KW + w) * 32 + (h & 7) * 4 + qc) * (2 * NQ);
-        dst[0] = *reinterpret_cast<const uint32_t*>(&p0), dst[1] = *reinterpret_cast<const uint32_t*>(&p1);
-        if constexpr (NQ == 2) {
-          dst[2] = half2_bits(a0 - __low2float(p0), a1 - __high2float(p0));
-          dst[3] = half2_bits(a2 - __low2float(p1), a3 - __high2float(p1));
+        for (int w4 = 0; w4 < 4; ++w4) {
+          const int qc = D >= 128 ? (ch & 7) >> 1 : D == 64 ? ch : 2 * ch + (w4 >> 1);
+          const int w = D >= 128 ? (ch >> 3) * 8 + (ch & 1) * 4 + w4 : D == 64 ? w4 : w4 & 1;
+          uint32_t b[NQ];
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) b[t] = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // (a tiny amax: M / amax overflows, so the element is scaled in two steps)
+            int v = top >= 1e-30f ? __float2int_rn(q[w4 * 4 + e] * up)
+                                  : amax ? __float2int_rn(__fdiv_rn(q[w4 * 4 + e], top) * M) : 0;
+#pragma unroll
+            for (int t = NQ - 1; t >= 0; --t) {  // the least significant byte last
+              const int lo = (int)(int8_t)(v & 0xff);
+              b[t] |= (uint32_t)(lo & 0xff) << (8 * e);
+              v = (v - lo) >> 8;
+            }
+          }
+          uint32_t* dst = reinterpret_cast<uint32_t*>(sm + C::kQ);
+#pragma unroll
+          for (int t = 0; t < NQ; ++t)
+            dst[((((h >> 3) * (KW / 2) + (w >> 1)) * NQ + t) * 32 + (h & 7) * 4 + qc) * 2 + (w & 1)] = b[t];
+        }
+      } else {
+        const int ex = min(max((int)(amax >> 23), 1), 253);  // biased exponent
+        const float down = __uint_as_float((uint32_t)(254 - ex) << 23);
+        if (ch == 0) qscale[h] = __uint_as_float((uint32_t)ex << 23) * base;
+#pragma unroll
+        for (int w4 = 0; w4 < 4; ++w4) {  // 4 dims: word w of thread (h % 8, qc)
+          const int qc = D >= 128 ? (ch & 7) >> 1 : D == 64 ? ch : 2 * ch + (w4 >> 1);
+          const int w = D >= 128 ? (ch >> 3) * 8 + (ch & 1) * 4 + w4 : D == 64 ? w4 : w4 & 1;
+          const float a0 = q[w4 * 4] * down, a1 = q[w4 * 4 + 1] * down, a2 = q[w4 * 4 + 2] * down, a3 = q[w4 * 4 + 3] * down;
+          const __half2 p0 = __floats2half2_rn(a0, a1), p1 = __floats2half2_rn(a2, a3);
+          uint32_t* dst = reinterpret_cast<uint32_t*>(sm + C::kQ) +
+                          (size_t)(((h >> 3) * KW + w) * 32 + (h & 7) * 4 + qc) * (2 * NQ);
+          dst[0] = *reinterpret_cast<const uint32_t*>(&p0), dst[1] = *reinterpret_cast<const uint32_t*>(&p1);
+          if constexpr (NQ == 2) {
+            dst[2] = half2_bits(a0 - __low2float(p0), a1 - __high2float(p0));
+            dst[3] = half2_bits(a2 - __low2float(p1), a3 - __high2float(p1));
+          }
         }
       }
     }
@@ -456,11 +494,53 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       const uint32_t valid_u = valid_q[0];
       issue(stage == 0 ? S - 1 : stage - 1);  // into the buffer that was consumed last
       const uint32_t buf = ring + stage * C::kStageBytes;
+      if constexpr (CT == kE4M3)
+        if (valid_u != (U == 32 ? 0xffffffffu : 0xffffu)) {  // what lies in rows without a key may be NaN codes: P = 0 times 0
+#pragma unroll
+          for (int t = 0; t < PER; ++t) {
+            const int r = (t * 32 + lane) / CH, ch = (t * 32 + lane) % CH;
+            if (!((valid_u >> r) & 1u))
+              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(buf + C::kData + swz<D>(r, ch)), "r"(0) : "memory");
+          }
+          __syncwarp();
+        }
 #pragma unroll 1
       for (int kt = 0; kt < NT; ++kt) {  // 16 keys
         const uint32_t valid = valid_u >> (kt * 16);
         const uint32_t sks = buf + 2 * C::kData + kt * 64, svs = sks + U * 4;
         float s[NT][4];
+        if constexpr (C::kInt) {
+          int si[NT][NQ][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int t = 0; t < NQ; ++t) si[nt][t][0] = si[nt][t][1] = si[nt][t][2] = si[nt][t][3] = 0;
+#pragma unroll
+          for (int wb = 0; wb < KW; wb += KV) {
+            uint32_t ka[KV], kb[KV];
+            const int r0 = kt * 16 + g, byte = kbyte<D>(c, wb);
+            lds<KV * 4>(buf + swz<D>(r0, byte >> 4) + (byte & 15), ka);
+            lds<KV * 4>(buf + swz<D>(r0 + 8, byte >> 4) + (byte & 15), kb);
+#pragma unroll
+            for (int w = 0; w < KV; w += 2)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int t = 0; t < NQ; ++t) {
+                  uint32_t b[2];
+                  lds<8>(smem_u32(sm) + C::kQ + (((nt * (KW / 2) + (wb + w) / 2) * NQ + t) * 32 + lane) * 8, b);
+                  mma_s8(si[nt][t], ka[w], kb[w], ka[w + 1], kb[w + 1], b[0], b[1]);
+                }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {  // |sums| <= D 127 128: 2^22 at D = 256, 2^30 after the shift
+              int v = si[nt][0][e] * 256 + si[nt][1][e];
+              if constexpr (NQ == 3) v += (si[nt][2][e] + 128) >> 8;
+              s[nt][e] = (float)v;
+            }
+        } else {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
@@ -482,6 +562,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
               for (int t = 0; t < NQ; ++t) mma(s[nt], a, b[2 * t], b[2 * t + 1]);
             }
           }
+        }
         }
         // scores in base 2: key g (r = 0) and g + 8 (r = 1), heads 2c and 2c + 1
         float vs[2];
@@ -590,9 +671,9 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
             for (int t = 0; t < MT; ++t)
               mg[merge_at<D>(hd, (vbyte<D>(g, t >> 1) >> 1) + (t & 1))] = make_float2(o[t][nt][h], o[t][nt][2 + h]);
         }
-      static_assert(kLift == 6, "the powers below");
+      static_assert(kLift == 6, "the power below");
       if (lane == 0)
-        misc[warp] = make_float2(__uint_as_float((uint32_t)E << 23) * (CT == kE4M3 ? 4.f : 0x1p-6f), __int_as_float(freeb));
+        misc[warp] = make_float2(__uint_as_float((uint32_t)E << 23) * 0x1p-6f, __int_as_float(freeb));
     }
     __syncthreads();
     const bool whole = nseg == at.nu;
@@ -675,7 +756,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
 
 template <typename T, int D, int CT, int NT>
 cudaError_t launch_t(const PagedQ8& a, bool appended, cudaStream_t st) {
-  using C = Cfg<T, D, NT>;
+  using C = Cfg<T, D, CT, NT>;
   auto kern = paged_q8_attn_kernel<T, D, CT, NT>;
   if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kTotal)) return e;
   const int grid = std::min(a.ctas, num_sms() * C::kCtasPerSm);
