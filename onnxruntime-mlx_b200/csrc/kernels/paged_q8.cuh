@@ -11,7 +11,8 @@
 
 namespace b200ep {
 
-enum { kErrPagedQ8 = 122 };  // a position or page outside the tables (detail: packed row or sequence)
+// a position or page outside the tables (detail: packed row or sequence); a bounded wait that ran out
+enum { kErrPagedQ8 = 122, kErrPagedQ8Timeout = 123 };
 enum { kI8 = 3, kE4M3 = 17 };  // cache_type: ONNX TensorProto INT8 / FLOAT8E4M3FN
 
 struct PagedQ8 {

@@ -37,6 +37,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr int kRowTab = 64;
 constexpr int kLift = 6;       // P vs is held times 2^kLift
 constexpr float kSlack = 8.f;  // a score may pass the running maximum by this much (in base 2) before it moves
 
@@ -56,7 +57,8 @@ struct Cfg {
   static constexpr int kMl = kQ + kQBytes;                        // [kWarps][kHeads] (m, l)
   static constexpr int kScale = kMl + kWarps * kHeads * 8;        // [kHeads] score factor
   static constexpr int kMisc = kScale + kHeads * 4;               // [kWarps] (output factor, buffer)
-  static constexpr int kTotal = kMisc + kWarps * 8;
+  static constexpr int kRaw = kMisc + kWarps * 8;                 // the next segment's q rows, cos and sin row
+  static constexpr int kStatic = 768;                             // (bound on the static shared memory)
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -194,7 +196,7 @@ template <typename T>
 __device__ __forceinline__ void load16(const T* p, float (&x)[16]) {
   uint4 w[sizeof(T)];
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(T); ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  for (int i = 0; i < (int)sizeof(T); ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
   const T* h = reinterpret_cast<const T*>(w);
 #pragma unroll
   for (int e = 0; e < 16; ++e) x[e] = to_f<T>(h[e]);
@@ -219,14 +221,20 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
   constexpr int MT = D / 16;  // 16-dim tiles of the output
   constexpr int KV = KW >= 4 ? 4 : KW, VV = VW >= 4 ? 4 : VW;  // words of one load
   extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ uint64_t qbar;
   __shared__ long long plan_s;
   __shared__ int scan_s[kWarps], plan_i, flag_s;
+  __shared__ int2 row_s[kRowTab];  // (keys, sequence) of the rows from the run's first on
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const uint32_t ring = smem_u32(sm) + warp * S * C::kStageBytes;
   float2* mls = reinterpret_cast<float2*>(sm + C::kMl);
   float* qscale = reinterpret_cast<float*>(sm + C::kScale);
   float2* misc = reinterpret_cast<float2*>(sm + C::kMisc);
   const int HC = kp.HK * hchunks;
+  if (tid == 0) {
+    mbar_init(&qbar, 1);
+    fence_mbarrier_init();
+  }
   bool waited = false;
   if (appended) {  // the launch before this one wrote rows that are read here
     pdl_wait();
@@ -260,10 +268,11 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
   }
   const long long w0 = W * cta / ctas;
   const int run = (int)(W * (cta + 1) / ctas - w0);
+  int tab_n;  // entries of row_s
   {
     long long base = 0;
-    for (int i0 = 0; i0 < kp.ntok; i0 += kThreads) {
-      const int i = i0 + tid, n = i0 ? row_keys(kp, i, seq0) : n0;
+    for (int i0 = 0;; i0 += kThreads) {
+      const int i = i0 + tid, n = i0 || kp.ntok > kThreads ? row_keys(kp, i, seq0) : n0;
       const int nu = (n + U - 1) / U;
       int inc = nu;
 #pragma unroll
@@ -280,12 +289,27 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       }
       if (nu && pre * HC <= w0 && w0 < (pre + nu) * HC) plan_i = i, plan_s = pre * HC;
       __syncthreads();
-      if (base * HC > w0) break;
+      if (base * HC > w0) {
+        const int j = i - plan_i;
+        if (j >= 0 && j < kRowTab) row_s[j] = make_int2(n, seq0);
+        tab_n = min(kRowTab, i0 + kThreads - plan_i);
+        break;
+      }
     }
+    __syncthreads();
   }
   // a position in the unit list: unit u of head chunk hc of row `row`, which has nu units (n keys)
   struct Pos {
     int row, seq, n, nu, hc, u;
+  };
+  const int tab0 = plan_i;
+  auto keys_of = [&](int row, int& seq) {
+    if (row - tab0 < tab_n) {
+      const int2 v = row_s[row - tab0];
+      seq = v.y;
+      return v.x;
+    }
+    return row_keys(kp, row, seq);
   };
   auto settle = [&](Pos& p) {  // carries u past the head chunks and rows that it has left
     while (p.u >= p.nu) {
@@ -294,7 +318,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
         p.hc = 0;
         do {
           ++p.row;
-          p.n = row_keys(kp, p.row, p.seq);
+          p.n = keys_of(p.row, p.seq);
         } while (p.n == 0 && p.row < kp.ntok);
         p.nu = p.row < kp.ntok ? (p.n + U - 1) / U : 0x7fffffff;  // (past the last row: nothing more is issued)
       }
@@ -302,13 +326,31 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
   };
   Pos at;  // the segment in work
   at.row = plan_i;
-  at.n = row_keys(kp, at.row, at.seq);
+  at.n = keys_of(at.row, at.seq);
   at.nu = (at.n + U - 1) / U;
   {
     const long long off = w0 - plan_s;
     at.hc = (int)(off / at.nu);
     at.u = (int)(off % at.nu);
   }
+
+  // ---- q rows of a segment, and the cos / sin row of its position, on their way to shared memory (one
+  // thread; aligned rows only)
+  T* raw = reinterpret_cast<T*>(sm + C::kRaw);
+  auto fetch_q = [&](const Pos& p) {
+    const int ck = hchunks == 1 ? 0 : p.hc % hchunks, nh = min(C::kHeads, kp.G - ck * C::kHeads);
+    const int first = (hchunks == 1 ? p.hc : p.hc / hchunks) * kp.G + ck * C::kHeads;
+    const uint32_t qb = nh * D * sizeof(T), cb = kp.rot ? kp.half * sizeof(T) : 0;
+    mbar_arrive_expect_tx(&qbar, qb + 2 * cb);
+    bulk_g2s(raw, static_cast<const T*>(kp.q) + (size_t)p.row * kp.qs + (size_t)first * D, qb, &qbar);
+    if (cb) {
+      T* cs = raw + min(C::kHeads, kp.G) * D;
+      bulk_g2s(cs, static_cast<const T*>(kp.cos_c) + (size_t)(p.n - 1) * kp.half, cb, &qbar);
+      bulk_g2s(cs + kp.half, static_cast<const T*>(kp.sin_c) + (size_t)(p.n - 1) * kp.half, cb, &qbar);
+    }
+  };
+  if ((vec & 1) && tid == 0) fetch_q(at);
+  uint32_t qphase = 0;
 
   // ---- the warp's stream: units warp, warp + 4, ... of the run, S - 1 ahead of their use
   Pos is = at;
@@ -391,6 +433,13 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
     const int chunk = hchunks == 1 ? 0 : at.hc % hchunks;
     const int h0 = (hchunks == 1 ? at.hc : at.hc / hchunks) * kp.G + chunk * C::kHeads;  // first query head
     const int heads = min(C::kHeads, kp.G - chunk * C::kHeads);
+    Pos nx = at;  // the segment after this one
+    nx.u += nseg;
+    if (x + nseg < run) settle(nx);
+    if (vec & 1) {
+      if (!mbar_wait(&qbar, qphase) && tid == 0) report_device_error(kp.err, kErrPagedQ8Timeout, at.row);
+      qphase ^= 1;
+    }
     // ---- q as the second operand, in shared memory: 16 dims of a head per thread, D / 16 threads a head
     constexpr uint32_t kQLanes = C::kHeads * CH >= 32 ? 0xffffffffu : 0xffffu;  // (16 or a multiple of 32 threads)
     if (tid < C::kHeads * CH) {
@@ -401,14 +450,15 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       if (h < heads) {
         const T* row = static_cast<const T*>(kp.q) + (size_t)at.row * kp.qs + (size_t)(h0 + h) * D;
         if (vec & 1) {  // aligned rows, halves of whole 16-dim chunks
-          load16<T>(row + d0, q);
+          load16<T>(raw + h * D + d0, q);
           if (kp.rot && d0 < 2 * kp.half) {
             const bool first = d0 < kp.half;
             const int i0 = first ? d0 : d0 - kp.half;
+            const T* cs_row = raw + min(C::kHeads, kp.G) * D;
             float y[16], cs[16], sn[16];
-            load16<T>(row + (first ? d0 + kp.half : i0), y);
-            load16<T>(static_cast<const T*>(kp.cos_c) + (size_t)pos * kp.half + i0, cs);
-            load16<T>(static_cast<const T*>(kp.sin_c) + (size_t)pos * kp.half + i0, sn);
+            load16<T>(raw + h * D + (first ? d0 + kp.half : i0), y);
+            load16<T>(cs_row + i0, cs);
+            load16<T>(cs_row + kp.half + i0, sn);
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               q[e] = first ? __fsub_rn(__fmul_rn(q[e], cs[e]), __fmul_rn(y[e], sn[e]))
@@ -476,7 +526,8 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
         }
       }
     }
-    __syncthreads();  // q is there; the merge buffers of the segment before are free
+    __syncthreads();  // q is there; the merge buffers of the segment before, and the raw rows, are free
+    if ((vec & 1) && tid == 0 && x + nseg < run) fetch_q(nx);
 
     float o[MT][NT][4], m[NT][2], l[NT][2];
     int E = kLift + 1;  // biased exponent that P vs is relative to
@@ -721,33 +772,56 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       if (flag_s) {  // the last to arrive joins the parts, in the order of the keys
         __threadfence();
         const size_t step = (size_t)2 * C::kHeads * (D + 2);  // from one run's first part to the next one's
-        const float* first = kp.part + (size_t)(2 * kf + 1) * C::kHeads * (D + 2);
         const float* rest = kp.part + (size_t)(2 * kf) * C::kHeads * (D + 2);
-        for (int e = tid; e < heads * (D / 4); e += kThreads) {
-          const int hd = e / (D / 4), d = (e % (D / 4)) * 4;
-          float mm = __ldcg(first + C::kHeads * D + hd * 2);
+        const int parts = kl - kf + 1;
+        auto part_at = [&](int k) { return rest + (k ? k * step : step / 2); };
+        constexpr int KC = D / 2;  // parts at a time: their (m, l) fit a merge buffer
+        constexpr int IT = C::kHeads * D / 4 / kThreads > 0 ? C::kHeads * D / 4 / kThreads : 1;
+        float2* mlb = reinterpret_cast<float2*>(sm + __float_as_int(misc[0].y) * C::kStageBytes);
+        float mm[IT], ll[IT];
+        float4 acc[IT];
+#pragma unroll
+        for (int i = 0; i < IT; ++i) mm[i] = -INFINITY, ll[i] = 0.f, acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < parts; k0 += KC) {
+          const int nk = min(KC, parts - k0);
+          __syncthreads();
+          for (int e = tid; e < nk * C::kHeads; e += kThreads)
+            if (e % C::kHeads < heads)
+              mlb[e] = __ldcg(reinterpret_cast<const float2*>(part_at(k0 + e / C::kHeads) + C::kHeads * D) + e % C::kHeads);
+          __syncthreads();
+#pragma unroll
+          for (int i = 0; i < IT; ++i) {
+            const int e = tid + i * kThreads;
+            if (e >= heads * (D / 4)) break;
+            const int hd = e / (D / 4), d = (e % (D / 4)) * 4;
+            float mn = mm[i];
+            for (int k = 0; k < nk; ++k) mn = fmaxf(mn, mlb[k * C::kHeads + hd].x);
+            const float a0 = ll[i] == 0.f ? 0.f : ex2(mm[i] - mn);
+            mm[i] = mn, ll[i] *= a0;
+            acc[i].x *= a0, acc[i].y *= a0, acc[i].z *= a0, acc[i].w *= a0;
 #pragma unroll 8
-          for (int k = 1; k <= kl - kf; ++k) mm = fmaxf(mm, __ldcg(rest + k * step + C::kHeads * D + hd * 2));
-          float ll = 0.f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int k = 0; k <= kl - kf; ++k) {
-            const float* pp = k ? rest + k * step : first;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(pp + C::kHeads * D + hd * 2));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(pp + hd * D + d));
-            const float f = ml.y == 0.f ? 0.f : ex2(ml.x - mm);
-            ll += ml.y * f;
-            acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+            for (int k = 0; k < nk; ++k) {
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(part_at(k0 + k) + hd * D + d));
+              const float2 ml = mlb[k * C::kHeads + hd];
+              const float f = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
+              ll[i] += ml.y * f;
+              acc[i].x += v.x * f, acc[i].y += v.y * f, acc[i].z += v.z * f, acc[i].w += v.w * f;
+            }
           }
-          const float r = ll == 0.f ? 0.f : __frcp_rn(ll);
-          T* q = out + hd * D + d;
-          q[0] = from_f<T>(acc.x * r), q[1] = from_f<T>(acc.y * r), q[2] = from_f<T>(acc.z * r), q[3] = from_f<T>(acc.w * r);
+        }
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+          const int e = tid + i * kThreads;
+          if (e >= heads * (D / 4)) break;
+          const float r = ll[i] == 0.f ? 0.f : __frcp_rn(ll[i]);
+          T* q = out + (e / (D / 4)) * D + (e % (D / 4)) * 4;
+          q[0] = from_f<T>(acc[i].x * r), q[1] = from_f<T>(acc[i].y * r);
+          q[2] = from_f<T>(acc[i].z * r), q[3] = from_f<T>(acc[i].w * r);
         }
       }
     }
     x += nseg;
-    at.u += nseg;
-    if (x < run) settle(at);
+    at = nx;
   }
   cp_wait<0>();
   if (__any_sync(0xffffffffu, bad) && lane == 0) report_device_error(kp.err, kErrPagedQ8, at.row);
@@ -758,8 +832,11 @@ template <typename T, int D, int CT, int NT>
 cudaError_t launch_t(const PagedQ8& a, bool appended, cudaStream_t st) {
   using C = Cfg<T, D, CT, NT>;
   auto kern = paged_q8_attn_kernel<T, D, CT, NT>;
-  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kTotal)) return e;
-  const int grid = std::min(a.ctas, num_sms() * C::kCtasPerSm);
+  const int smem = C::kRaw + (std::min(a.G, C::kHeads) * D + (a.rot ? 2 * a.half : 0)) * (int)sizeof(T);
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
+  // one wave: the CTAs that the SM's 228 KB hold (1 KB of each is the system's)
+  const int per_sm = std::min<int>(C::kCtasPerSm, 228 * 1024 / (smem + C::kStatic + 1024));
+  const int grid = std::min(a.ctas, num_sms() * per_sm);
   if (!appended)
     if (cudaError_t e = launch_k(paged_q8_reset_kernel, dim3(1), dim3(256), 0, st, a.counters, grid)) return e;
   const int hchunks = (a.G + C::kHeads - 1) / C::kHeads;
@@ -768,7 +845,7 @@ cudaError_t launch_t(const PagedQ8& a, bool appended, cudaStream_t st) {
   int vec = al(a.q, a.qs * es) &&
             (!a.rot || (!a.inter && a.half % 16 == 0 && al(a.cos_c, (int64_t)a.half * es) && al(a.sin_c, 0)));
   if (al(a.kscale, 0) && al(a.vscale, 0)) vec |= 2;
-  return launch_k(kern, dim3((unsigned)grid), dim3(kThreads), C::kTotal, st, a, hchunks, appended ? 1 : 0, vec);
+  return launch_k(kern, dim3((unsigned)grid), dim3(kThreads), smem, st, a, hchunks, appended ? 1 : 0, vec);
 }
 
 template <typename T, int D, int CT>
