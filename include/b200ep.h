@@ -266,7 +266,7 @@ B200EP_API int b200ep_paged_kv_dequantize(const b200ep_paged_q8_params* p, const
 
 /* Attention over the 8-bit cache.  Row j of sequence b sees positions 0 .. past_seqlens[b] + j; its
  * query is RoPE'd here.  With key / value (both, or neither) the new rows are first written as by
- * b200ep_paged_kv_quantize.  out [num_tokens, num_heads * head_size].  Meant for one or a few new
+ * b200ep_paged_kv_quantize.  out [num_tokens, num_heads * head_size], 16-byte aligned.  Meant for one or a few new
  * tokens per sequence: every row reads its keys on its own, so a long prompt is better attended by
  * reading its past back (b200ep_paged_kv_dequantize) and b200ep_group_query_attention.
  * workspace: b200ep_paged_attention_quantized_workspace_size(p) bytes (num_heads, kv_heads and

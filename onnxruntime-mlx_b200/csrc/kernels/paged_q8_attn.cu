@@ -151,55 +151,36 @@ __device__ __forceinline__ float lds_f(uint32_t addr) {
   return v;
 }
 
-// Element d of query row x after RoPE at position pos, in fp32.
+// Element d of query row x after RoPE by the row (cs, sn), in fp32.
 template <typename T>
-__device__ __forceinline__ float q_at(const T* x, int d, const PagedQ8& kp, int pos) {
+__device__ __forceinline__ float q_at(const T* x, int d, const PagedQ8& kp, const T* cs, const T* sn) {
   const float v = to_f<T>(x[d]);
   if (!kp.rot || d >= 2 * kp.half) return v;
-  int pi, o;
-  bool first;
-  if (kp.inter) {
-    first = !(d & 1), pi = d >> 1, o = d ^ 1;
-  } else {
-    first = d < kp.half, pi = first ? d : d - kp.half, o = first ? d + kp.half : pi;
-  }
-  const float c = to_f<T>(static_cast<const T*>(kp.cos_c)[(size_t)pos * kp.half + pi]);
-  const float s = to_f<T>(static_cast<const T*>(kp.sin_c)[(size_t)pos * kp.half + pi]);
-  const float y = to_f<T>(x[o]);
-  return first ? __fsub_rn(__fmul_rn(v, c), __fmul_rn(y, s)) : __fadd_rn(__fmul_rn(v, c), __fmul_rn(y, s));
+  const bool first = kp.inter ? !(d & 1) : d < kp.half;
+  const int pi = kp.inter ? d >> 1 : first ? d : d - kp.half;
+  const float y = to_f<T>(x[kp.inter ? d ^ 1 : first ? d + kp.half : pi]), c = to_f<T>(cs[pi]), s = to_f<T>(sn[pi]);
+  const float a = __fmul_rn(v, c), b = __fmul_rn(y, s);
+  return first ? __fsub_rn(a, b) : __fadd_rn(a, b);
 }
 
-// Keys that row i sees (0: none, an invalid row) and its sequence.
-__device__ __forceinline__ int row_keys(const PagedQ8& kp, int i, int& seq) {
-  seq = -1;
-  if (i >= kp.ntok) return 0;
-  int past = i < kp.batch ? __ldg(kp.past + i) : 0, first = i;  // (one new token per sequence: row i is sequence i)
-  if (i < kp.batch && __ldg(kp.cum + i) == i && __ldg(kp.cum + i + 1) == i + 1) {
-    seq = i;
-  } else {
-    seq = q8_seq(kp.cum, kp.batch, i);
-    if (seq < 0) return 0;
-    past = __ldg(kp.past + seq), first = __ldg(kp.cum + seq);
+// Keys that row i sees (0: none, an invalid row) and its sequence.  Out of line: it is needed in many places, and
+// what runs once per CTA costs instruction fetches.
+__device__ __noinline__ int2 row_keys(const int32_t* cum, const int32_t* past_, int ntok, int batch, int most, int i) {
+  if (i >= ntok) return make_int2(0, -1);
+  int seq = i, past = i < batch ? __ldg(past_ + i) : 0, first = i;  // (one new token per sequence: row i is sequence i)
+  if (!(i < batch && __ldg(cum + i) == i && __ldg(cum + i + 1) == i + 1)) {
+    seq = q8_seq(cum, batch, i);
+    if (seq < 0) return make_int2(0, -1);
+    past = __ldg(past_ + seq), first = __ldg(cum + seq);
   }
   const int pos = past + (i - first);
-  return pos < 0 || pos >= (int64_t)kp.maxb * kp.bs || (kp.rot && pos >= kp.max_seq) ? 0 : pos + 1;
+  return make_int2(pos < 0 || pos >= most ? 0 : pos + 1, seq);
 }
 
 __global__ void paged_q8_reset_kernel(int* counters, int n) {
   pdl_wait();
   pdl_trigger();
   for (int t = threadIdx.x; t < n; t += blockDim.x) counters[t] = 0;
-}
-
-// 16 consecutive elements at a 16-byte aligned address
-template <typename T>
-__device__ __forceinline__ void load16(const T* p, float (&x)[16]) {
-  uint4 w[sizeof(T)];
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T); ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
-  const T* h = reinterpret_cast<const T*>(w);
-#pragma unroll
-  for (int e = 0; e < 16; ++e) x[e] = to_f<T>(h[e]);
 }
 
 // Pair p (dims 2p, 2p + 1) of head h in a warp's [kHeads][D] merge buffer: the 16 lanes that store at
@@ -209,6 +190,15 @@ __device__ __forceinline__ int merge_at(int h, int p) {
   const int c = (h >> 1) & 3;
   const int f = D >= 128 ? ((p >> 4) & 1) | (c << 1) : D == 64 ? c : (c & 1) | ((c >> 1) << 3);
   return h * (D / 2) + (p ^ f);
+}
+
+// acc / l to four elements of the output (0 where no key was seen)
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, float4 a, float l) {
+  const float r = l == 0.f ? 0.f : __frcp_rn(l);
+  alignas(4 * sizeof(T)) T v[4] = {from_f<T>(a.x * r), from_f<T>(a.y * r), from_f<T>(a.z * r), from_f<T>(a.w * r)};
+  if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(v);
+  else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
 }
 
 template <typename T, int D, int CT, int NT>
@@ -241,39 +231,24 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
     waited = true;
   }
 
-  // ---- this CTA's run [w0, w1) of the unit list, and the row that w0 lies in
-  long long total = 0;
-  int seq0, n0 = row_keys(kp, tid, seq0);
-  for (int i0 = 0; i0 < kp.ntok; i0 += kThreads) {
-    const int i = i0 + tid, n = i0 ? row_keys(kp, i, seq0) : n0;
-    if (i < kp.ntok && n == 0 && i % (int)gridDim.x == (int)blockIdx.x) {
-      if (!waited) pdl_wait();  // an earlier launch may still use `out`
-      T* o = static_cast<T*>(kp.out) + (size_t)i * kp.H * D;
-      for (int e = 0; e < kp.H * D; ++e) o[e] = from_f<T>(0.f);
-      report_device_error(kp.err, kErrPagedQ8, i);
-    }
-    const int s = __reduce_add_sync(0xffffffffu, (n + U - 1) / U);
-    if (lane == 0) scan_s[warp] = s;
-    __syncthreads();
-    for (int w = 0; w < kWarps; ++w) total += scan_s[w];
-    __syncthreads();
-  }
-  const long long W = total * HC;
-  const int ctas = (int)max(1ll, min((long long)gridDim.x, (W + kWarps - 1) / kWarps));
+  // positions that a row may have: inside the block table, and inside the cos / sin rows
+  const int most = (int)min((int64_t)kp.maxb * kp.bs, (int64_t)(kp.rot ? kp.max_seq : 0x7fffffff));
+  auto keys_at = [&](int i) { return row_keys(kp.cum, kp.past, kp.ntok, kp.batch, most, i); };
+  for (int i = tid; i < (C::kQBytes + 4 * C::kHeads) / 4; i += kThreads)  // heads that a group lacks: q = 0
+    (i < C::kQBytes / 4 ? reinterpret_cast<uint32_t*>(sm + C::kQ)[i]
+                        : reinterpret_cast<uint32_t*>(sm + C::kScale)[i - C::kQBytes / 4]) = 0;
+
+  // ---- this CTA's run of the unit list: every CTA counts all units, then looks for the row of its first
+  long long W = 0, w0 = 0, per = 0, rem = 0;
+  int run = 0, ctas = 1, tab_n = 0;
   const int cta = blockIdx.x;
-  if (W == 0 || cta >= ctas) {
-    if (!waited) pdl_wait();
-    pdl_trigger();
-    return;
-  }
-  const long long w0 = W * cta / ctas;
-  const int run = (int)(W * (cta + 1) / ctas - w0);
-  int tab_n;  // entries of row_s
-  {
+  for (int pass = 0; pass < 2; ++pass) {
     long long base = 0;
-    for (int i0 = 0;; i0 += kThreads) {
-      const int i = i0 + tid, n = i0 || kp.ntok > kThreads ? row_keys(kp, i, seq0) : n0;
-      const int nu = (n + U - 1) / U;
+#pragma unroll 1
+    for (int i0 = 0; i0 < kp.ntok; i0 += kThreads) {
+      const int i = i0 + tid;
+      const int2 r = keys_at(i);
+      const int nu = (r.x + U - 1) / U;
       int inc = nu;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -287,30 +262,40 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
         if (w < warp) pre += scan_s[w];
         base += scan_s[w];
       }
-      if (nu && pre * HC <= w0 && w0 < (pre + nu) * HC) plan_i = i, plan_s = pre * HC;
+      if (pass && nu && pre * HC <= w0 && w0 < (pre + nu) * HC) plan_i = i, plan_s = pre * HC;
       __syncthreads();
-      if (base * HC > w0) {
+      if (pass && base * HC > w0) {
         const int j = i - plan_i;
-        if (j >= 0 && j < kRowTab) row_s[j] = make_int2(n, seq0);
+        if (j >= 0 && j < kRowTab) row_s[j] = r;
         tab_n = min(kRowTab, i0 + kThreads - plan_i);
         break;
       }
+      if (!pass && i < kp.ntok && r.x == 0 && i % (int)gridDim.x == cta) {  // an invalid row
+        if (!waited) pdl_wait();  // an earlier launch may still use `out`
+        for (int e = 0; e < kp.H * D; ++e) static_cast<T*>(kp.out)[(size_t)i * kp.H * D + e] = from_f<T>(0.f);
+        report_device_error(kp.err, kErrPagedQ8, i);
+      }
     }
-    __syncthreads();
+    if (!pass) {
+      W = base * HC;
+      ctas = (int)max(1ll, min((long long)gridDim.x, (W + kWarps - 1) / kWarps));
+      if (W == 0 || cta >= ctas) {
+        if (!waited) pdl_wait();
+        pdl_trigger();
+        return;
+      }
+      per = W / ctas, rem = W - per * ctas;  // the first rem runs have one unit more
+      w0 = cta * per + min((long long)cta, rem);
+      run = (int)per + (cta < rem);
+    }
   }
+  __syncthreads();
   // a position in the unit list: unit u of head chunk hc of row `row`, which has nu units (n keys)
   struct Pos {
     int row, seq, n, nu, hc, u;
   };
   const int tab0 = plan_i;
-  auto keys_of = [&](int row, int& seq) {
-    if (row - tab0 < tab_n) {
-      const int2 v = row_s[row - tab0];
-      seq = v.y;
-      return v.x;
-    }
-    return row_keys(kp, row, seq);
-  };
+  auto keys_of = [&](int row) { return row - tab0 < tab_n ? row_s[row - tab0] : keys_at(row); };
   auto settle = [&](Pos& p) {  // carries u past the head chunks and rows that it has left
     while (p.u >= p.nu) {
       p.u -= p.nu;
@@ -318,20 +303,21 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
         p.hc = 0;
         do {
           ++p.row;
-          p.n = keys_of(p.row, p.seq);
+          const int2 r = keys_of(p.row);
+          p.n = r.x, p.seq = r.y;
         } while (p.n == 0 && p.row < kp.ntok);
         p.nu = p.row < kp.ntok ? (p.n + U - 1) / U : 0x7fffffff;  // (past the last row: nothing more is issued)
       }
     }
   };
   Pos at;  // the segment in work
-  at.row = plan_i;
-  at.n = keys_of(at.row, at.seq);
+  at.row = tab0;
+  at.n = row_s[0].x, at.seq = row_s[0].y;
   at.nu = (at.n + U - 1) / U;
   {
-    const long long off = w0 - plan_s;
+    const long long off = w0 - plan_s;  // < nu HC
     at.hc = (int)(off / at.nu);
-    at.u = (int)(off % at.nu);
+    at.u = (int)(off - (long long)at.hc * at.nu);
   }
 
   // ---- q rows of a segment, and the cos / sin row of its position, on their way to shared memory (one
@@ -394,7 +380,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       } else {
         bad |= row < 0 && lane < U && lane < left;
         valid = __ballot_sync(0xffffffffu, row >= 0);
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < PER; ++t) {
           const int r = (t * 32 + lane) / CH, ch = (t * 32 + lane) % CH;
           const int src = __shfl_sync(0xffffffffu, row, r);
@@ -440,88 +426,76 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       if (!mbar_wait(&qbar, qphase) && tid == 0) report_device_error(kp.err, kErrPagedQ8Timeout, at.row);
       qphase ^= 1;
     }
-    // ---- q as the second operand, in shared memory: 16 dims of a head per thread, D / 16 threads a head
-    constexpr uint32_t kQLanes = C::kHeads * CH >= 32 ? 0xffffffffu : 0xffffu;  // (16 or a multiple of 32 threads)
-    if (tid < C::kHeads * CH) {
-      const int h = tid / CH, ch = tid % CH, d0 = ch * 16, pos = at.n - 1;
-      float q[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) q[e] = 0.f;
-      if (h < heads) {
-        const T* row = static_cast<const T*>(kp.q) + (size_t)at.row * kp.qs + (size_t)(h0 + h) * D;
-        if (vec & 1) {  // aligned rows, halves of whole 16-dim chunks
-          load16<T>(raw + h * D + d0, q);
-          if (kp.rot && d0 < 2 * kp.half) {
-            const bool first = d0 < kp.half;
-            const int i0 = first ? d0 : d0 - kp.half;
-            const T* cs_row = raw + min(C::kHeads, kp.G) * D;
-            float y[16], cs[16], sn[16];
-            load16<T>(raw + h * D + (first ? d0 + kp.half : i0), y);
-            load16<T>(cs_row + i0, cs);
-            load16<T>(cs_row + kp.half + i0, sn);
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              q[e] = first ? __fsub_rn(__fmul_rn(q[e], cs[e]), __fmul_rn(y[e], sn[e]))
-                           : __fadd_rn(__fmul_rn(q[e], cs[e]), __fmul_rn(y[e], sn[e]));
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) q[e] = q_at<T>(row, d0 + e, kp, pos);
-        }
-      }
+    else {
+      const T* src = static_cast<const T*>(kp.q) + (size_t)at.row * kp.qs + (size_t)h0 * D;
+#pragma unroll 1
+      for (int e = tid; e < heads * D; e += kThreads) raw[e] = src[e];
+      if (kp.rot)
+#pragma unroll 1
+        for (int e = tid; e < 2 * kp.half; e += kThreads)
+          raw[min(C::kHeads, kp.G) * D + e] =
+              (e < kp.half ? static_cast<const T*>(kp.cos_c) + e : static_cast<const T*>(kp.sin_c) + e - kp.half)
+                  [(size_t)(at.n - 1) * kp.half];
+      __syncthreads();
+    }
+    // ---- q as the second operand, in shared memory: a head per LPH lanes
+    constexpr int LPH = D / 4 < 32 ? D / 4 : 32, EPL = D / LPH, HPW = 32 / LPH;
+#pragma unroll 1
+    for (int hb = warp * HPW; hb < heads; hb += kWarps * HPW) {
+      const int h = hb + lane / LPH, d0 = (lane % LPH) * EPL;
+      const bool on = h < heads;
+      const T* cs = raw + min(C::kHeads, kp.G) * D;
+      float q[EPL];
       uint32_t amax = 0;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) amax = max(amax, __float_as_uint(q[e]) & 0x7fffffffu);
+      for (int e = 0; e < EPL; ++e) {
+        q[e] = on ? q_at<T>(raw + h * D, d0 + e, kp, cs, cs + kp.half) : 0.f;
+        amax = max(amax, __float_as_uint(q[e]) & 0x7fffffffu);
+      }
 #pragma unroll
-      for (int o = CH / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(kQLanes, amax, o));
+      for (int o = LPH / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (!on) continue;
       const float base = kp.scale * 1.4426950408889634f;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(sm + C::kQ);
+      const bool finite = amax < 0x7f800000u;
+      float mul;  // what q is multiplied by
       if constexpr (C::kInt) {
         // q / amax as an integer of kNQ bytes, each in [-128, 127]
-        const float top = __uint_as_float(amax), M = NQ == 3 ? 127.f * 65536.f : 127.f * 256.f;
-        const float up = amax && amax < 0x7f800000u ? __fdiv_rn(M, top) : 0.f;
-        if (ch == 0)  // what the sum in units of the upper two bytes' last place stands for
-          qscale[h] = amax < 0x7f800000u ? top * base * (NQ == 3 ? 256.f / (127.f * 65536.f) : 1.f / (127.f * 256.f))
-                                         : __uint_as_float(0x7fc00000u);
-#pragma unroll
-        for (int w4 = 0; w4 < 4; ++w4) {
-          const int qc = D >= 128 ? (ch & 7) >> 1 : D == 64 ? ch : 2 * ch + (w4 >> 1);
-          const int w = D >= 128 ? (ch >> 3) * 8 + (ch & 1) * 4 + w4 : D == 64 ? w4 : w4 & 1;
-          uint32_t b[NQ];
-#pragma unroll
-          for (int t = 0; t < NQ; ++t) b[t] = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            // (a tiny amax: M / amax overflows, so the element is scaled in two steps)
-            int v = top >= 1e-30f ? __float2int_rn(q[w4 * 4 + e] * up)
-                                  : amax ? __float2int_rn(__fdiv_rn(q[w4 * 4 + e], top) * M) : 0;
-#pragma unroll
-            for (int t = NQ - 1; t >= 0; --t) {  // the least significant byte last
-              const int lo = (int)(int8_t)(v & 0xff);
-              b[t] |= (uint32_t)(lo & 0xff) << (8 * e);
-              v = (v - lo) >> 8;
-            }
-          }
-          uint32_t* dst = reinterpret_cast<uint32_t*>(sm + C::kQ);
-#pragma unroll
-          for (int t = 0; t < NQ; ++t)
-            dst[((((h >> 3) * (KW / 2) + (w >> 1)) * NQ + t) * 32 + (h & 7) * 4 + qc) * 2 + (w & 1)] = b[t];
-        }
+        constexpr float M = NQ == 3 ? 127.f * 65536.f : 127.f * 256.f;
+        const float top = fmaxf(__uint_as_float(amax), 1e-30f);  // (all below: q rounds to 0, as its scores would)
+        mul = __fdiv_rn(M, top);
+        if (lane % LPH == 0)  // what the sum, in units of the upper two bytes' last place, stands for
+          qscale[h] = finite ? top * base * ((NQ == 3 ? 256.f : 1.f) / M) : __uint_as_float(0x7fc00000u);
       } else {
         const int ex = min(max((int)(amax >> 23), 1), 253);  // biased exponent
-        const float down = __uint_as_float((uint32_t)(254 - ex) << 23);
-        if (ch == 0) qscale[h] = __uint_as_float((uint32_t)ex << 23) * base;
+        mul = __uint_as_float((uint32_t)(254 - ex) << 23);
+        if (lane % LPH == 0) qscale[h] = __uint_as_float((uint32_t)ex << 23) * base;
+      }
 #pragma unroll
-        for (int w4 = 0; w4 < 4; ++w4) {  // 4 dims: word w of thread (h % 8, qc)
-          const int qc = D >= 128 ? (ch & 7) >> 1 : D == 64 ? ch : 2 * ch + (w4 >> 1);
-          const int w = D >= 128 ? (ch >> 3) * 8 + (ch & 1) * 4 + w4 : D == 64 ? w4 : w4 & 1;
-          const float a0 = q[w4 * 4] * down, a1 = q[w4 * 4 + 1] * down, a2 = q[w4 * 4 + 2] * down, a3 = q[w4 * 4 + 3] * down;
+      for (int j = 0; j < EPL / 4; ++j) {  // 4 dims: word w of thread (h % 8, qc)
+        const int ch = (d0 + 4 * j) >> 4, w4 = ((d0 + 4 * j) >> 2) & 3;
+        const int qc = D >= 128 ? (ch & 7) >> 1 : D == 64 ? ch : 2 * ch + (w4 >> 1);
+        const int w = D >= 128 ? (ch >> 3) * 8 + (ch & 1) * 4 + w4 : D == 64 ? w4 : w4 & 1;
+        const int to = (h & 7) * 4 + qc;
+        if constexpr (C::kInt) {
+          uint32_t u[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)  // every byte lifted by 128: no carries between them
+            u[e] = (uint32_t)__float2int_rn(finite ? q[4 * j + e] * mul : 0.f) + (NQ == 3 ? 0x808080u : 0x8080u);
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) {
+            const int bi = NQ - 1 - t;  // the most significant byte first
+            const uint32_t a = prmt(u[0], u[1], (4 + bi) << 4 | bi), b = prmt(u[2], u[3], (4 + bi) << 4 | bi);
+            dst[((((h >> 3) * (KW / 2) + (w >> 1)) * NQ + t) * 32 + to) * 2 + (w & 1)] = prmt(a, b, 0x5410) ^ 0x80808080u;
+          }
+        } else {
+          const float a0 = q[4 * j] * mul, a1 = q[4 * j + 1] * mul, a2 = q[4 * j + 2] * mul, a3 = q[4 * j + 3] * mul;
           const __half2 p0 = __floats2half2_rn(a0, a1), p1 = __floats2half2_rn(a2, a3);
-          uint32_t* dst = reinterpret_cast<uint32_t*>(sm + C::kQ) +
-                          (size_t)(((h >> 3) * KW + w) * 32 + (h & 7) * 4 + qc) * (2 * NQ);
-          dst[0] = *reinterpret_cast<const uint32_t*>(&p0), dst[1] = *reinterpret_cast<const uint32_t*>(&p1);
+          uint32_t* o = dst + (((h >> 3) * KW + w) * 32 + to) * (2 * NQ);
+          o[0] = *reinterpret_cast<const uint32_t*>(&p0), o[1] = *reinterpret_cast<const uint32_t*>(&p1);
           if constexpr (NQ == 2) {
-            dst[2] = half2_bits(a0 - __low2float(p0), a1 - __high2float(p0));
-            dst[3] = half2_bits(a2 - __low2float(p1), a3 - __high2float(p1));
+            o[2] = half2_bits(a0 - __low2float(p0), a1 - __high2float(p0));
+            o[3] = half2_bits(a2 - __low2float(p1), a3 - __high2float(p1));
           }
         }
       }
@@ -735,88 +709,85 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
     T* out = static_cast<T*>(kp.out) + (size_t)at.row * kp.H * D + (size_t)h0 * D;
     const int slot = 2 * cta + (at.u > 0 ? 0 : 1);
     float* part = kp.part + (size_t)slot * C::kHeads * (D + 2);
-    for (int e = tid; e < heads * (D / 2); e += kThreads) {
-      const int hd = e / (D / 2), p = e % (D / 2);
-      float2 ml[kWarps], acc = make_float2(0.f, 0.f);
+#pragma unroll 1
+    for (int e = tid; e < heads * (D / 4); e += kThreads) {  // 4 dims of a head
+      const int hd = e / (D / 4), d = (e % (D / 4)) * 4;
       float mm = -INFINITY, ll = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, mls[w * C::kHeads + hd].x);
+      const int at2 = merge_at<D>(hd, d / 2), at3 = merge_at<D>(hd, d / 2 + 1);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        ml[w] = mls[w * C::kHeads + hd];
-        mm = fmaxf(mm, ml[w].x);
-      }
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (ml[w].y == 0.f) continue;  // the warp saw no key of this segment (a NaN is not 0)
-        const float2 us = misc[w];
-        const float f = ex2(ml[w].x - mm);
-        const float2 v = reinterpret_cast<const float2*>(sm + (w * S + __float_as_int(us.y)) * C::kStageBytes)[merge_at<D>(hd, p)];
-        ll += ml[w].y * f;
-        acc.x += v.x * (f * us.x), acc.y += v.y * (f * us.x);
+        const float2 ml = mls[w * C::kHeads + hd], us = misc[w];
+        const float f = ml.y == 0.f ? 0.f : ex2(ml.x - mm);  // 0: the warp saw no key of this segment (a NaN is not 0)
+        const float2* mg = reinterpret_cast<const float2*>(sm + (w * S + __float_as_int(us.y)) * C::kStageBytes);
+        ll += ml.y * f;
+        if (f != 0.f) {  // (else the buffer holds something else)
+          const float2 a = mg[at2], b = mg[at3];
+          acc.x += a.x * (f * us.x), acc.y += a.y * (f * us.x), acc.z += b.x * (f * us.x), acc.w += b.y * (f * us.x);
+        }
       }
       if (whole) {
-        const float r = ll == 0.f ? 0.f : __frcp_rn(ll);
-        out[hd * D + 2 * p] = from_f<T>(acc.x * r), out[hd * D + 2 * p + 1] = from_f<T>(acc.y * r);
+        store4<T>(out + hd * D + d, acc, ll);
       } else {
-        *reinterpret_cast<float2*>(part + hd * D + 2 * p) = acc;
-        if (p == 0) *reinterpret_cast<float2*>(part + C::kHeads * D + hd * 2) = make_float2(mm, ll);
+        *reinterpret_cast<float4*>(part + hd * D + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(part + C::kHeads * D + hd * 2) = make_float2(mm, ll);
       }
     }
     if (!whole) {
-      __threadfence();
-      __syncthreads();
       // the runs that hold units of this (row, head chunk); in the first of them it is the last segment
-      const long long a = w0 + x - at.u, z = a + at.nu;
-      const int kf = (int)(((a + 1) * ctas - 1) / W), kl = (int)((z * ctas - 1) / W);
-      if (tid == 0) flag_s = atomicAdd(kp.counters + kf, 1) == kl - kf;
+      auto run_of = [&](long long unit) {
+        const long long big = rem * (per + 1);
+        return (int)(unit < big ? unit / (per + 1) : rem + (unit - big) / per);
+      };
+      const long long a = w0 + x - at.u;
+      const int kf = run_of(a), parts = run_of(a + at.nu - 1) - kf + 1;
+      __syncthreads();
+      if (tid == 0) {
+        __threadfence();  // (orders what the whole CTA wrote before the barrier)
+        flag_s = atomicAdd(kp.counters + kf, 1) == parts - 1;
+        __threadfence();
+      }
       __syncthreads();
       if (flag_s) {  // the last to arrive joins the parts, in the order of the keys
-        __threadfence();
         const size_t step = (size_t)2 * C::kHeads * (D + 2);  // from one run's first part to the next one's
-        const float* rest = kp.part + (size_t)(2 * kf) * C::kHeads * (D + 2);
-        const int parts = kl - kf + 1;
-        auto part_at = [&](int k) { return rest + (k ? k * step : step / 2); };
+        const float* first = kp.part + (size_t)(2 * kf) * C::kHeads * (D + 2);
+        auto part_at = [&](int k) { return first + (k ? k * step : step / 2); };
         constexpr int KC = D / 2;  // parts at a time: their (m, l) fit a merge buffer
-        constexpr int IT = C::kHeads * D / 4 / kThreads > 0 ? C::kHeads * D / 4 / kThreads : 1;
         float2* mlb = reinterpret_cast<float2*>(sm + __float_as_int(misc[0].y) * C::kStageBytes);
-        float mm[IT], ll[IT];
-        float4 acc[IT];
-#pragma unroll
-        for (int i = 0; i < IT; ++i) mm[i] = -INFINITY, ll[i] = 0.f, acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k0 = 0; k0 < parts; k0 += KC) {
-          const int nk = min(KC, parts - k0);
-          __syncthreads();
-          for (int e = tid; e < nk * C::kHeads; e += kThreads)
-            if (e % C::kHeads < heads)
-              mlb[e] = __ldcg(reinterpret_cast<const float2*>(part_at(k0 + e / C::kHeads) + C::kHeads * D) + e % C::kHeads);
-          __syncthreads();
-#pragma unroll
-          for (int i = 0; i < IT; ++i) {
-            const int e = tid + i * kThreads;
-            if (e >= heads * (D / 4)) break;
-            const int hd = e / (D / 4), d = (e % (D / 4)) * 4;
-            float mn = mm[i];
+#pragma unroll 1
+        for (int e0 = 0; e0 < heads * (D / 4); e0 += kThreads) {
+          const int e = e0 + tid;
+          const bool on = e < heads * (D / 4);
+          const int hd = on ? e / (D / 4) : 0, d = (e % (D / 4)) * 4;
+          float mm = -INFINITY, ll = 0.f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+          for (int k0 = 0; k0 < parts; k0 += KC) {
+            const int nk = min(KC, parts - k0);
+            __syncthreads();
+#pragma unroll 1
+            for (int i = tid; i < nk * C::kHeads; i += kThreads)
+              if (i % C::kHeads < heads)
+                mlb[i] = __ldcg(reinterpret_cast<const float2*>(part_at(k0 + i / C::kHeads) + C::kHeads * D) + i % C::kHeads);
+            __syncthreads();
+            float mn = mm;
+#pragma unroll 4
             for (int k = 0; k < nk; ++k) mn = fmaxf(mn, mlb[k * C::kHeads + hd].x);
-            const float a0 = ll[i] == 0.f ? 0.f : ex2(mm[i] - mn);
-            mm[i] = mn, ll[i] *= a0;
-            acc[i].x *= a0, acc[i].y *= a0, acc[i].z *= a0, acc[i].w *= a0;
+            const float a0 = ll == 0.f ? 0.f : ex2(mm - mn);
+            mm = mn, ll *= a0;
+            acc.x *= a0, acc.y *= a0, acc.z *= a0, acc.w *= a0;
 #pragma unroll 8
             for (int k = 0; k < nk; ++k) {
               const float4 v = __ldcg(reinterpret_cast<const float4*>(part_at(k0 + k) + hd * D + d));
               const float2 ml = mlb[k * C::kHeads + hd];
               const float f = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
-              ll[i] += ml.y * f;
-              acc[i].x += v.x * f, acc[i].y += v.y * f, acc[i].z += v.z * f, acc[i].w += v.w * f;
+              ll += ml.y * f;
+              acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
             }
           }
-        }
-#pragma unroll
-        for (int i = 0; i < IT; ++i) {
-          const int e = tid + i * kThreads;
-          if (e >= heads * (D / 4)) break;
-          const float r = ll[i] == 0.f ? 0.f : __frcp_rn(ll[i]);
-          T* q = out + (e / (D / 4)) * D + (e % (D / 4)) * 4;
-          q[0] = from_f<T>(acc[i].x * r), q[1] = from_f<T>(acc[i].y * r);
-          q[2] = from_f<T>(acc[i].z * r), q[3] = from_f<T>(acc[i].w * r);
+          if (on) store4<T>(out + hd * D + d, acc, ll);
         }
       }
     }
@@ -843,7 +814,7 @@ cudaError_t launch_t(const PagedQ8& a, bool appended, cudaStream_t st) {
   auto al = [](const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && bytes % 16 == 0; };
   const int es = (int)sizeof(T);
   int vec = al(a.q, a.qs * es) &&
-            (!a.rot || (!a.inter && a.half % 16 == 0 && al(a.cos_c, (int64_t)a.half * es) && al(a.sin_c, 0)));
+            (!a.rot || (al(a.cos_c, (int64_t)a.half * es) && al(a.sin_c, 0)));
   if (al(a.kscale, 0) && al(a.vscale, 0)) vec |= 2;
   return launch_k(kern, dim3((unsigned)grid), dim3(kThreads), smem, st, a, hchunks, appended ? 1 : 0, vec);
 }

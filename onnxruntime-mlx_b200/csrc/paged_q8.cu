@@ -134,6 +134,7 @@ extern "C" B200EP_API int b200ep_paged_attention_quantized(
     B200EP_CHECK_ARG((!p->query_stride || p->query_stride >= (int64_t)p->num_heads * p->head_size) &&
                          (!p->key_stride || p->key_stride >= dense) && (!p->value_stride || p->value_stride >= dense),
                      "PagedAttentionQuantized: row strides must be at least heads * head_size");
+    B200EP_CHECK_ARG(aligned(out, nullptr, 16), "PagedAttentionQuantized: out must be 16-byte aligned");
     const size_t need = b200ep_paged_attention_quantized_workspace_size(p);
     B200EP_CHECK_ARG(workspace && workspace_bytes >= need && aligned(workspace, nullptr, 16),
                      "PagedAttentionQuantized: a 16-byte aligned workspace of " + std::to_string(need) +
