@@ -47,6 +47,7 @@ struct Cfg {
   static constexpr int kNQ = kInt + (std::is_same<T, __nv_bfloat16>::value ? 1 : 2);
   static constexpr int kNP = std::is_same<T, float>::value ? 2 : 1;          // fp16 terms of P
   static constexpr int kUnit = 16 * NT;  // keys of a unit
+  static constexpr int kOver = 8 / NT;   // units that a segment's start and end are counted as
   static constexpr int kHeads = 8 * NT;  // query heads of a CTA
   static constexpr int kStages = D >= 128 ? 3 : D == 64 ? 5 : 8;
   static constexpr int kCtasPerSm = D == 256 || NT == 2 ? 2 : std::is_same<T, float>::value ? 3 : 4;
@@ -212,9 +213,11 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
   constexpr int KV = KW >= 4 ? 4 : KW, VV = VW >= 4 ? 4 : VW;  // words of one load
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ uint64_t qbar;
-  __shared__ long long plan_s;
-  __shared__ int scan_s[kWarps], plan_i, flag_s;
+  __shared__ long long plan_s, real0_s, real1_s, per_s, rem_s, scan_s[kWarps];
+  __shared__ int plan_i, flag_s, tab0_s, tab_n_s, most_s;
   __shared__ int2 row_s[kRowTab];  // (keys, sequence) of the rows from the run's first on
+  __shared__ int4 seg_s[2];        // (row, keys, head chunk, first unit) of this segment and the next
+  __shared__ uint32_t valid_s[kWarps][S];  // keys of the units in flight, a bit each
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const uint32_t ring = smem_u32(sm) + warp * S * C::kStageBytes;
   float2* mls = reinterpret_cast<float2*>(sm + C::kMl);
@@ -225,99 +228,124 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
     mbar_init(&qbar, 1);
     fence_mbarrier_init();
   }
-  bool waited = false;
-  if (appended) {  // the launch before this one wrote rows that are read here
-    pdl_wait();
-    waited = true;
-  }
+  if (appended) pdl_wait();  // the launch before this one wrote rows that are read here
 
   // positions that a row may have: inside the block table, and inside the cos / sin rows
-  const int most = (int)min((int64_t)kp.maxb * kp.bs, (int64_t)(kp.rot ? kp.max_seq : 0x7fffffff));
-  auto keys_at = [&](int i) { return row_keys(kp.cum, kp.past, kp.ntok, kp.batch, most, i); };
+  if (tid == 0) most_s = (int)min((int64_t)kp.maxb * kp.bs, (int64_t)(kp.rot ? kp.max_seq : 0x7fffffff));
+  __syncthreads();
+  auto keys_at = [&](int i) { return row_keys(kp.cum, kp.past, kp.ntok, kp.batch, most_s, i); };
   for (int i = tid; i < (C::kQBytes + 4 * C::kHeads) / 4; i += kThreads)  // heads that a group lacks: q = 0
     (i < C::kQBytes / 4 ? reinterpret_cast<uint32_t*>(sm + C::kQ)[i]
                         : reinterpret_cast<uint32_t*>(sm + C::kScale)[i - C::kQBytes / 4]) = 0;
 
-  // ---- this CTA's run of the unit list: every CTA counts all units, then looks for the row of its first
-  long long W = 0, w0 = 0, per = 0, rem = 0;
-  int run = 0, ctas = 1, tab_n = 0;
+  // ---- this CTA's run of the unit list.  A (row, head chunk) of nu units weighs nu + kOver, the first kOver
+  // of which stand for its start; all CTAs get the same weight.  Every CTA adds up all rows, then looks for the
+  // two ends of its run.
+  constexpr int OV = C::kOver;
+  long long W = 0, w0 = 0, w1 = 0, per = 0, rem = 0;
+  int ctas = 1, tab_n = 0;
   const int cta = blockIdx.x;
+  const bool once = kp.ntok <= kThreads;  // one row per thread: the second pass needs no loads
+  int2 r = keys_at(tid);
+#pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
-    long long base = 0;
+    long long base = 0;  // units and, above them, rows with keys
 #pragma unroll 1
     for (int i0 = 0; i0 < kp.ntok; i0 += kThreads) {
       const int i = i0 + tid;
-      const int2 r = keys_at(i);
+      if (!once) r = keys_at(i);
       const int nu = (r.x + U - 1) / U;
-      int inc = nu;
+      const long long own = nu ? nu + (1ll << 40) : 0;
+      long long inc = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, inc, o);
+        const long long t = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += t;
       }
+      __syncthreads();
       if (lane == 31) scan_s[warp] = inc;
       __syncthreads();
-      long long pre = base + inc - nu;
+      long long pre = base + inc - own;
+#pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         if (w < warp) pre += scan_s[w];
         base += scan_s[w];
       }
-      if (pass && nu && pre * HC <= w0 && w0 < (pre + nu) * HC) plan_i = i, plan_s = pre * HC;
-      __syncthreads();
-      if (pass && base * HC > w0) {
+      constexpr long long kUnits = (1ll << 40) - 1;
+      if (pass && nu) {
+        const long long units = (pre & kUnits) * HC, v = units + (pre >> 40) * OV * HC;  // before this row
+        const long long end = v + (long long)(nu + OV) * HC;
+        auto real = [&](long long w) {  // units before weight w of this row
+          const int hc = (int)((w - v) / (nu + OV)), off = (int)(w - v - (long long)hc * (nu + OV));
+          return units + (long long)hc * nu + max(0, off - OV);
+        };
+        if (v <= w0 && w0 < end) plan_i = i, plan_s = v, real0_s = real(w0);
+        if (v < w1 && w1 <= end) real1_s = real(w1);
+      }
+      if (pass && ((base & kUnits) + (base >> 40) * OV) * HC > w0 && !tab_n) {
+        __syncthreads();
         const int j = i - plan_i;
         if (j >= 0 && j < kRowTab) row_s[j] = r;
         tab_n = min(kRowTab, i0 + kThreads - plan_i);
-        break;
       }
+      if (pass && ((base & kUnits) + (base >> 40) * OV) * HC >= w1) break;
       if (!pass && i < kp.ntok && r.x == 0 && i % (int)gridDim.x == cta) {  // an invalid row
-        if (!waited) pdl_wait();  // an earlier launch may still use `out`
+        pdl_wait();  // an earlier launch may still use `out`
+#pragma unroll 1
         for (int e = 0; e < kp.H * D; ++e) static_cast<T*>(kp.out)[(size_t)i * kp.H * D + e] = from_f<T>(0.f);
         report_device_error(kp.err, kErrPagedQ8, i);
       }
     }
     if (!pass) {
-      W = base * HC;
-      ctas = (int)max(1ll, min((long long)gridDim.x, (W + kWarps - 1) / kWarps));
+      W = ((base & ((1ll << 40) - 1)) + (base >> 40) * OV) * HC;
+      // (a run of more than kOver holds at least one unit)
+      ctas = (int)max(1ll, min((long long)gridDim.x, W / (OV + kWarps)));
       if (W == 0 || cta >= ctas) {
-        if (!waited) pdl_wait();
+        pdl_wait();
         pdl_trigger();
         return;
       }
-      per = W / ctas, rem = W - per * ctas;  // the first rem runs have one unit more
+      per = W / ctas, rem = W - per * ctas;  // the first rem runs weigh one more
       w0 = cta * per + min((long long)cta, rem);
-      run = (int)per + (cta < rem);
+      w1 = w0 + per + (cta < rem);
     }
   }
+  if (tid == 0) per_s = per, rem_s = rem, tab0_s = plan_i, tab_n_s = tab_n;
   __syncthreads();
-  // a position in the unit list: unit u of head chunk hc of row `row`, which has nu units (n keys)
+  const int run = (int)(real1_s - real0_s);
+  // a position in the unit list: unit u of head chunk hc of row `row`, which has n keys
   struct Pos {
-    int row, seq, n, nu, hc, u;
+    int row, seq, n, hc, u;
   };
-  const int tab0 = plan_i;
-  auto keys_of = [&](int row) { return row - tab0 < tab_n ? row_s[row - tab0] : keys_at(row); };
   auto settle = [&](Pos& p) {  // carries u past the head chunks and rows that it has left
-    while (p.u >= p.nu) {
-      p.u -= p.nu;
+    int nu = (p.n + U - 1) / U;
+    while (p.u >= nu) {
+      p.u -= nu;
       if (++p.hc == HC) {
         p.hc = 0;
+        int2 r;
         do {
           ++p.row;
-          const int2 r = keys_of(p.row);
-          p.n = r.x, p.seq = r.y;
-        } while (p.n == 0 && p.row < kp.ntok);
-        p.nu = p.row < kp.ntok ? (p.n + U - 1) / U : 0x7fffffff;  // (past the last row: nothing more is issued)
+          r = p.row - tab0_s < tab_n_s ? row_s[p.row - tab0_s] : keys_at(p.row);
+        } while (r.x == 0 && p.row < kp.ntok);
+        p.n = r.x, p.seq = r.y;
+        nu = p.row < kp.ntok ? (p.n + U - 1) / U : 0x7fffffff;  // (past the last row: nothing is issued)
       }
     }
   };
-  Pos at;  // the segment in work
-  at.row = tab0;
-  at.n = row_s[0].x, at.seq = row_s[0].y;
-  at.nu = (at.n + U - 1) / U;
+  Pos is;  // of the warp's next unit to issue; first the run's first unit
+  is.row = tab0_s;
+  is.n = row_s[0].x, is.seq = row_s[0].y;
   {
-    const long long off = w0 - plan_s;  // < nu HC
-    at.hc = (int)(off / at.nu);
-    at.u = (int)(off - (long long)at.hc * at.nu);
+    const int nv = (is.n + U - 1) / U + OV;
+    const long long off = w0 - plan_s;  // < nv HC
+    is.hc = (int)(off / nv);
+    is.u = max(0, (int)(off - (long long)is.hc * nv) - OV);
+    __syncthreads();
+    if (tid == 0) {
+      seg_s[0] = make_int4(is.row, is.n, is.hc, is.u);
+      plan_s += (long long)is.hc * nv;  // from here: the weight before the segment's (row, head chunk)
+    }
   }
 
   // ---- q rows of a segment, and the cos / sin row of its position, on their way to shared memory (one
@@ -335,35 +363,31 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       bulk_g2s(cs + kp.half, static_cast<const T*>(kp.sin_c) + (size_t)(p.n - 1) * kp.half, cb, &qbar);
     }
   };
-  if ((vec & 1) && tid == 0) fetch_q(at);
+  if ((vec & 1) && tid == 0) fetch_q(is);
   uint32_t qphase = 0;
 
   // ---- the warp's stream: units warp, warp + 4, ... of the run, S - 1 ahead of their use
-  Pos is = at;
   is.u += warp;
   settle(is);
-  int ix = warp;  // next unit to issue, within the run
   // whole units lie in one page (16-row aligned): one lookup a unit, else one a key
   const bool paged = kp.bs % U == 0 && (vec & 2);
-  auto lookup = [&]() -> int {
+  auto lookup = [&](int ix) -> int {
     if (ix >= run) return -1;
     const int key = is.u * U + (paged ? 0 : lane);
     return key < is.n && (paged || lane < U)
                ? q8_row(kp.bt, kp.maxb, kp.nblocks, kp.bs, kp.HK, is.seq, hchunks == 1 ? is.hc : is.hc / hchunks, key)
                : -1;
   };
-  int next_row = lookup();
-  bool bad = false;
-  uint32_t valid_q[S - 1];  // of the units in flight, the oldest first
+  int next_row = lookup(warp);
   constexpr int CH = D / 16, PER = U * CH / 32;  // 16-byte chunks of a row; of a unit's K per lane
-  auto issue = [&](int stage) {
+  auto issue = [&](int stage, int ix) {  // unit ix of the run into buffer `stage`
     uint32_t valid = 0;
     if (ix < run) {
       const int row = next_row, left = is.n - is.u * U;  // keys from this unit's first on
       const uint32_t dst = ring + stage * C::kStageBytes;
       const uint32_t inside = left >= U ? (U == 32 ? 0xffffffffu : 0xffffu) : (1u << left) - 1u;
       if (paged) {
-        bad |= row < 0;
+        if (row < 0 && lane == 0) report_device_error(kp.err, kErrPagedQ8, is.row);
         if (row >= 0) {
           valid = inside;
           const size_t o = (size_t)row * D + lane * 16;
@@ -378,7 +402,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
           else if (lane < U / 2) cp16(dst + 2 * C::kData + lane * 16, kp.vscale + row + (lane - U / 4) * 4);
         }
       } else {
-        bad |= row < 0 && lane < U && lane < left;
+        if (row < 0 && lane < U && lane < left) report_device_error(kp.err, kErrPagedQ8, is.row);
         valid = __ballot_sync(0xffffffffu, row >= 0);
 #pragma unroll 1
         for (int t = 0; t < PER; ++t) {
@@ -396,38 +420,32 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
           cp4(dst + 2 * C::kData + U * 4 + lane * 4, kp.vscale + row);
         }
       }
-      ix += kWarps;
       is.u += kWarps;
-      if (ix < run) settle(is);
-      next_row = lookup();
+      if (ix + kWarps < run) settle(is);
+      next_row = lookup(ix + kWarps);
     }
     cp_commit();
-#pragma unroll
-    for (int i = 0; i + 1 < S - 1; ++i) valid_q[i] = valid_q[i + 1];
-    valid_q[S - 2] = valid;
+    if (lane == 0) valid_s[warp][stage] = valid;
   };
-#pragma unroll
-  for (int i = 0; i < S - 1; ++i) valid_q[i] = 0;
 #pragma unroll 1
-  for (int i = 0; i < S - 1; ++i) issue(i);
+  for (int i = 0; i < S - 1; ++i) issue(i, warp + i * kWarps);
 
   int stage = 0;
   int x = 0;        // first unit of the segment, within the run
   int mine = warp;  // the warp's next unit
+  int par = 0;  // which of seg_s
   while (x < run) {
-    const int nseg = min(at.nu - at.u, run - x);  // units of this segment
-    const int chunk = hchunks == 1 ? 0 : at.hc % hchunks;
-    const int h0 = (hchunks == 1 ? at.hc : at.hc / hchunks) * kp.G + chunk * C::kHeads;  // first query head
+    const int4 sg = seg_s[par];  // row, keys, head chunk, first unit
+    const int nseg = min((sg.y + U - 1) / U - sg.w, run - x);  // units of this segment
+    const int chunk = hchunks == 1 ? 0 : sg.z % hchunks;
+    const int h0 = (hchunks == 1 ? sg.z : sg.z / hchunks) * kp.G + chunk * C::kHeads;  // first query head
     const int heads = min(C::kHeads, kp.G - chunk * C::kHeads);
-    Pos nx = at;  // the segment after this one
-    nx.u += nseg;
-    if (x + nseg < run) settle(nx);
     if (vec & 1) {
-      if (!mbar_wait(&qbar, qphase) && tid == 0) report_device_error(kp.err, kErrPagedQ8Timeout, at.row);
+      if (!mbar_wait(&qbar, qphase) && tid == 0) report_device_error(kp.err, kErrPagedQ8Timeout, sg.x);
       qphase ^= 1;
     }
     else {
-      const T* src = static_cast<const T*>(kp.q) + (size_t)at.row * kp.qs + (size_t)h0 * D;
+      const T* src = static_cast<const T*>(kp.q) + (size_t)sg.x * kp.qs + (size_t)h0 * D;
 #pragma unroll 1
       for (int e = tid; e < heads * D; e += kThreads) raw[e] = src[e];
       if (kp.rot)
@@ -435,7 +453,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
         for (int e = tid; e < 2 * kp.half; e += kThreads)
           raw[min(C::kHeads, kp.G) * D + e] =
               (e < kp.half ? static_cast<const T*>(kp.cos_c) + e : static_cast<const T*>(kp.sin_c) + e - kp.half)
-                  [(size_t)(at.n - 1) * kp.half];
+                  [(size_t)(sg.y - 1) * kp.half];
       __syncthreads();
     }
     // ---- q as the second operand, in shared memory: a head per LPH lanes
@@ -501,7 +519,12 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       }
     }
     __syncthreads();  // q is there; the merge buffers of the segment before, and the raw rows, are free
-    if ((vec & 1) && tid == 0 && x + nseg < run) fetch_q(nx);
+    if (tid == 0 && x + nseg < run) {
+      Pos nx{sg.x, 0, sg.y, sg.z, sg.w + nseg};
+      settle(nx);
+      seg_s[par ^ 1] = make_int4(nx.row, nx.n, nx.hc, nx.u);
+      if (vec & 1) fetch_q(nx);
+    }
 
     float o[MT][NT][4], m[NT][2], l[NT][2];
     int E = kLift + 1;  // biased exponent that P vs is relative to
@@ -516,8 +539,8 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
     for (; mine < x + nseg; mine += kWarps) {
       cp_wait<S - 2>();
       __syncwarp();
-      const uint32_t valid_u = valid_q[0];
-      issue(stage == 0 ? S - 1 : stage - 1);  // into the buffer that was consumed last
+      const uint32_t valid_u = valid_s[warp][stage];
+      issue(stage == 0 ? S - 1 : stage - 1, mine + (S - 1) * kWarps);  // into the buffer that was consumed last
       const uint32_t buf = ring + stage * C::kStageBytes;
       if constexpr (CT == kE4M3)
         if (valid_u != (U == 32 ? 0xffffffffu : 0xffffu)) {  // what lies in rows without a key may be NaN codes: P = 0 times 0
@@ -701,13 +724,12 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
         misc[warp] = make_float2(__uint_as_float((uint32_t)E << 23) * 0x1p-6f, __int_as_float(freeb));
     }
     __syncthreads();
-    const bool whole = nseg == at.nu;
-    if (!waited) {  // before anything is written
-      pdl_wait();
-      waited = true;
-    }
-    T* out = static_cast<T*>(kp.out) + (size_t)at.row * kp.H * D + (size_t)h0 * D;
-    const int slot = 2 * cta + (at.u > 0 ? 0 : 1);
+    pdl_wait();  // before anything is written
+    const int4 sw = seg_s[par];
+    const int nu = (sw.y + U - 1) / U;
+    const bool whole = nseg == nu;
+    T* out = static_cast<T*>(kp.out) + (size_t)sw.x * kp.H * D + (size_t)h0 * D;
+    const int slot = 2 * cta + (sw.w > 0 ? 0 : 1);
     float* part = kp.part + (size_t)slot * C::kHeads * (D + 2);
 #pragma unroll 1
     for (int e = tid; e < heads * (D / 4); e += kThreads) {  // 4 dims of a head
@@ -737,22 +759,24 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
     }
     if (!whole) {
       // the runs that hold units of this (row, head chunk); in the first of them it is the last segment
-      auto run_of = [&](long long unit) {
-        const long long big = rem * (per + 1);
-        return (int)(unit < big ? unit / (per + 1) : rem + (unit - big) / per);
+      auto run_of = [&](long long w) {
+        const long long n = per_s, m = rem_s, big = m * (n + 1);
+        return (int)(w < big ? w / (n + 1) : m + (w - big) / n);
       };
-      const long long a = w0 + x - at.u;
-      const int kf = run_of(a), parts = run_of(a + at.nu - 1) - kf + 1;
       __syncthreads();
       if (tid == 0) {
+        const long long a = plan_s + OV;  // weight before the first unit
+        const int kf = run_of(a), parts = run_of(a + nu - 1) - kf + 1;
         __threadfence();  // (orders what the whole CTA wrote before the barrier)
-        flag_s = atomicAdd(kp.counters + kf, 1) == parts - 1;
+        flag_s = atomicAdd(kp.counters + kf, 1) == parts - 1 ? parts : 0;
         __threadfence();
+        plan_i = kf;
       }
       __syncthreads();
-      if (flag_s) {  // the last to arrive joins the parts, in the order of the keys
-        const size_t step = (size_t)2 * C::kHeads * (D + 2);  // from one run's first part to the next one's
-        const float* first = kp.part + (size_t)(2 * kf) * C::kHeads * (D + 2);
+      const int parts = flag_s, kf = plan_i;
+      if (parts) {  // the last to arrive joins the parts, in the order of the keys
+        constexpr int step = 2 * C::kHeads * (D + 2);  // from one run's first part to the next one's
+        const float* first = kp.part + kf * step;
         auto part_at = [&](int k) { return first + (k ? k * step : step / 2); };
         constexpr int KC = D / 2;  // parts at a time: their (m, l) fit a merge buffer
         float2* mlb = reinterpret_cast<float2*>(sm + __float_as_int(misc[0].y) * C::kStageBytes);
@@ -778,24 +802,35 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
             const float a0 = ll == 0.f ? 0.f : ex2(mm - mn);
             mm = mn, ll *= a0;
             acc.x *= a0, acc.y *= a0, acc.z *= a0, acc.w *= a0;
-#pragma unroll 8
-            for (int k = 0; k < nk; ++k) {
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(part_at(k0 + k) + hd * D + d));
-              const float2 ml = mlb[k * C::kHeads + hd];
-              const float f = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
-              ll += ml.y * f;
-              acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+            const float* pk = part_at(k0) + hd * D + d;
+            constexpr int MLP = 8;  // parts on their way at once
+#pragma unroll 1
+            for (int k = 0; k < nk; k += MLP) {
+              float4 v[MLP];
+#pragma unroll
+              for (int j = 0; j < MLP; ++j) {
+                if (k + j < nk) v[j] = __ldcg(reinterpret_cast<const float4*>(pk));
+                pk += k0 + k + j ? step : step / 2;
+              }
+#pragma unroll
+              for (int j = 0; j < MLP; ++j) {
+                if (k + j >= nk) break;
+                const float2 ml = mlb[(k + j) * C::kHeads + hd];
+                const float f = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
+                ll += ml.y * f;
+                acc.x += v[j].x * f, acc.y += v[j].y * f, acc.z += v[j].z * f, acc.w += v[j].w * f;
+              }
             }
           }
           if (on) store4<T>(out + hd * D + d, acc, ll);
         }
       }
     }
+    if (tid == 0 && sw.w + nseg == nu) plan_s += nu + OV;
     x += nseg;
-    at = nx;
+    par ^= 1;
   }
   cp_wait<0>();
-  if (__any_sync(0xffffffffu, bad) && lane == 0) report_device_error(kp.err, kErrPagedQ8, at.row);
   pdl_trigger();
 }
 
