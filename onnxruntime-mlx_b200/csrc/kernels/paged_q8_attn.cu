@@ -178,6 +178,11 @@ __device__ __noinline__ int2 row_keys(const int32_t* cum, const int32_t* past_, 
   return make_int2(pos < 0 || pos >= most ? 0 : pos + 1, seq);
 }
 
+// a / b for a >= 0, b > 0: almost always of 32-bit numbers
+__device__ __forceinline__ long long div64(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (uint32_t)a / (uint32_t)b : a / b;
+}
+
 __global__ void paged_q8_reset_kernel(int* counters, int n) {
   pdl_wait();
   pdl_trigger();
@@ -242,70 +247,77 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
   // of which stand for its start; all CTAs get the same weight.  Every CTA adds up all rows, then looks for the
   // two ends of its run.
   constexpr int OV = C::kOver;
-  long long W = 0, w0 = 0, w1 = 0, per = 0, rem = 0;
+  constexpr long long kUnits = (1ll << 40) - 1;  // sums hold units and, above them, rows with keys
+  long long W = 0, w0 = 0, w1 = 0, per = 0, rem = 0, pre = 0;
   int ctas = 1, tab_n = 0;
   const int cta = blockIdx.x;
-  const bool once = kp.ntok <= kThreads;  // one row per thread: the second pass needs no loads
+  const bool once = kp.ntok <= kThreads;  // one row per thread: the second pass has all it needs
   int2 r = keys_at(tid);
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
-    long long base = 0;  // units and, above them, rows with keys
+    long long base = 0;
 #pragma unroll 1
     for (int i0 = 0; i0 < kp.ntok; i0 += kThreads) {
       const int i = i0 + tid;
       if (!once) r = keys_at(i);
       const int nu = (r.x + U - 1) / U;
-      const long long own = nu ? nu + (1ll << 40) : 0;
-      long long inc = own;
+      if (!(pass && once)) {
+        const long long own = nu ? nu + (1ll << 40) : 0;
+        long long inc = own;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += t;
-      }
-      __syncthreads();
-      if (lane == 31) scan_s[warp] = inc;
-      __syncthreads();
-      long long pre = base + inc - own;
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long t = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += t;
+        }
+        __syncthreads();
+        if (lane == 31) scan_s[warp] = inc;
+        __syncthreads();
+        pre = base + inc - own;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) pre += scan_s[w];
-        base += scan_s[w];
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) pre += scan_s[w];
+          base += scan_s[w];
+        }
       }
-      constexpr long long kUnits = (1ll << 40) - 1;
-      if (pass && nu) {
+      if (!pass) {
+        if (i < kp.ntok && r.x == 0 && i % (int)gridDim.x == cta) {  // an invalid row
+          pdl_wait();  // an earlier launch may still use `out`
+#pragma unroll 1
+          for (int e = 0; e < kp.H * D; ++e) static_cast<T*>(kp.out)[(size_t)i * kp.H * D + e] = from_f<T>(0.f);
+          report_device_error(kp.err, kErrPagedQ8, i);
+        }
+        continue;
+      }
+      if (nu) {
         const long long units = (pre & kUnits) * HC, v = units + (pre >> 40) * OV * HC;  // before this row
-        const long long end = v + (long long)(nu + OV) * HC;
+        const int nv = nu + OV;
         auto real = [&](long long w) {  // units before weight w of this row
-          const int hc = (int)((w - v) / (nu + OV)), off = (int)(w - v - (long long)hc * (nu + OV));
+          const int hc = (int)div64(w - v, nv), off = (int)(w - v - (long long)hc * nv);
           return units + (long long)hc * nu + max(0, off - OV);
         };
+        const long long end = v + (long long)nv * HC;
         if (v <= w0 && w0 < end) plan_i = i, plan_s = v, real0_s = real(w0);
         if (v < w1 && w1 <= end) real1_s = real(w1);
       }
-      if (pass && ((base & kUnits) + (base >> 40) * OV) * HC > w0 && !tab_n) {
-        __syncthreads();
+      __syncthreads();
+      const long long done = once ? W : ((base & kUnits) + (base >> 40) * OV) * HC;
+      if (done > w0 && !tab_n) {
         const int j = i - plan_i;
         if (j >= 0 && j < kRowTab) row_s[j] = r;
         tab_n = min(kRowTab, i0 + kThreads - plan_i);
       }
-      if (pass && ((base & kUnits) + (base >> 40) * OV) * HC >= w1) break;
-      if (!pass && i < kp.ntok && r.x == 0 && i % (int)gridDim.x == cta) {  // an invalid row
-        pdl_wait();  // an earlier launch may still use `out`
-#pragma unroll 1
-        for (int e = 0; e < kp.H * D; ++e) static_cast<T*>(kp.out)[(size_t)i * kp.H * D + e] = from_f<T>(0.f);
-        report_device_error(kp.err, kErrPagedQ8, i);
-      }
+      if (done >= w1) break;
     }
     if (!pass) {
-      W = ((base & ((1ll << 40) - 1)) + (base >> 40) * OV) * HC;
+      W = ((base & kUnits) + (base >> 40) * OV) * HC;
       // (a run of more than kOver holds at least one unit)
-      ctas = (int)max(1ll, min((long long)gridDim.x, W / (OV + kWarps)));
+      ctas = (int)max(1ll, min((long long)gridDim.x, div64(W, OV + kWarps)));
       if (W == 0 || cta >= ctas) {
         pdl_wait();
         pdl_trigger();
         return;
       }
-      per = W / ctas, rem = W - per * ctas;  // the first rem runs weigh one more
+      per = div64(W, ctas), rem = W - per * ctas;  // the first rem runs weigh one more
       w0 = cta * per + min((long long)cta, rem);
       w1 = w0 + per + (cta < rem);
     }
@@ -339,7 +351,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
   {
     const int nv = (is.n + U - 1) / U + OV;
     const long long off = w0 - plan_s;  // < nv HC
-    is.hc = (int)(off / nv);
+    is.hc = (int)div64(off, nv);
     is.u = max(0, (int)(off - (long long)is.hc * nv) - OV);
     __syncthreads();
     if (tid == 0) {
@@ -761,7 +773,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       // the runs that hold units of this (row, head chunk); in the first of them it is the last segment
       auto run_of = [&](long long w) {
         const long long n = per_s, m = rem_s, big = m * (n + 1);
-        return (int)(w < big ? w / (n + 1) : m + (w - big) / n);
+        return (int)(w < big ? div64(w, n + 1) : m + div64(w - big, n));
       };
       __syncthreads();
       if (tid == 0) {
@@ -803,7 +815,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
             mm = mn, ll *= a0;
             acc.x *= a0, acc.y *= a0, acc.z *= a0, acc.w *= a0;
             const float* pk = part_at(k0) + hd * D + d;
-            constexpr int MLP = 8;  // parts on their way at once
+            constexpr int MLP = 6;  // parts on their way at once
 #pragma unroll 1
             for (int k = 0; k < nk; k += MLP) {
               float4 v[MLP];
