@@ -12,13 +12,18 @@
 //
 // One cluster of C CTAs per row; each CTA keeps its slice of the row in shared memory and every pass runs on
 // that copy: HBM sees the logits once, and the noise of kept tokens only.
-//   * The last kept token of top-k, and of top-p, is found by radix descent over the composite key
-//     (logit as an ordered integer, inverted index): 11 bits a round, counts (top-k) or masses (top-p) per
-//     digit summed over the cluster, until the digit's bucket is taken whole or holds one token.  The
-//     inverted index in the low bits settles ties.
-//   * Masses are summed as fixed-point integers, w 2^32 in two 16-bit halves: integer sums do not depend on
-//     the order of the atomics, so equal inputs give equal tokens.  Rounding is at most 2^-33 of the largest
-//     weight per token.
+//   * top-k: the k-th largest of the threads' own maxima is a lower bound of the k-th largest logit, and a close
+//     one.  A histogram of one value per thread gives it; the few tokens above go to the first CTA (at most
+//     kCap), which finishes the row alone: the rank and the mass before each token by comparison with every
+//     other, then top-k, top-p, min-p and the race.
+//   * top-p (and a top-k too large for that): tokens are split by d = M - x into 16 bins, then those of the bin
+//     that holds the border into 2048.  In the first split every thread adds its elements to bins of its own (a
+//     column of shared memory): no atomics, and fp32 sums that always add in the same order.  The tokens of the
+//     last bin, or all up to it where those are few, go to the first CTA, which finds the border; all CTAs race.
+//   * Rows that stay crowded (hundreds of equal logits at the border) go through radix descent over the composite
+//     key (logit as an ordered integer, inverted index), 11 bits a round, with integer atomics.
+//   * Masses of single tokens are summed as fixed-point integers (w 2^32 rounded, at most 2^-33 of the largest
+//     weight off per token), so no sum depends on the order of atomics: equal inputs give equal tokens.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -36,16 +41,26 @@ constexpr int kWarpsS = kThreads / 32;
 constexpr int kDigit = 11, kBins = 1 << kDigit;
 constexpr int kMaxCluster = 8;
 
+constexpr int kSplit = 16;   // bins of the first split: one warp adds up each
+constexpr int kCap = kThreads;  // tokens that one CTA finishes alone, one per thread
+constexpr int kTop = 128;    // bins of the threads' maxima
+static_assert(kSplit == kWarpsS && kCap <= kThreads, "one warp a bin, one thread a token");
+
+struct Token {
+  float x;
+  int index;
+};
+__device__ __forceinline__ bool before(Token a, Token b) { return a.x > b.x || (a.x == b.x && a.index < b.index); }
+
 struct Red {  // what CTAs of a cluster exchange; one slot per use, so that no barrier is needed before reuse
   float maxv, sum;
   unsigned long long mass, best;
+  float bin[2][kSplit];  // of the first split, by count and by mass
+  int top[kTop];
+  Token cut;             // written by the first CTA
+  int got;               // tokens collected
+  Token list[kCap];
 };
-
-template <typename T>
-__device__ __forceinline__ float logit(const T* p, int i) {
-  const float x = to_f<T>(p[i]);
-  return x == x ? x + 0.f : -INFINITY;  // NaN: never sampled; -0 and 0 are one value
-}
 
 // Ordered integer of a logit: 16 bits for 16-bit types, 32 for float.
 template <typename T>
@@ -63,10 +78,64 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return u;
 }
 
+// The logit with that ordered integer (below -infinity: -infinity).
+template <typename T>
+__device__ __forceinline__ float from_ordered(uint32_t u) {
+  float x;
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t h = (uint16_t)((u & 0x8000u) ? u & 0x7fffu : ~u);
+    T t;
+    memcpy(&t, &h, 2);
+    x = to_f<T>(t);
+  } else {
+    x = __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+  }
+  return x == x ? x : -INFINITY;
+}
+
 __device__ __forceinline__ unsigned long long fixed32(float w) {  // w in [0, 1] times 2^32, rounded
   const float h = w * 65536.f, hi = truncf(h);
   return ((unsigned long long)(uint32_t)hi << 16) + (unsigned long long)__float2uint_rn((h - hi) * 65536.f);
 }
+
+// 16 bytes of logits: NaN to -infinity, and the largest.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static __device__ __forceinline__ float clean(uint4& w) {
+    float* f = reinterpret_cast<float*>(&w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = fmaxf(f[j], -INFINITY);
+    return largest(w);
+  }
+  static __device__ __forceinline__ float largest(const uint4& w) {
+    const float* f = reinterpret_cast<const float*>(&w);
+    return fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+  }
+};
+template <typename T2>
+__device__ __forceinline__ T2 both(float v);
+template <>
+__device__ __forceinline__ __half2 both<__half2>(float v) { return __float2half2_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat162 both<__nv_bfloat162>(float v) { return __float2bfloat162_rn(v); }
+template <typename T2>
+struct Vec16 {
+  static __device__ __forceinline__ float clean(uint4& w) {
+    T2* h = reinterpret_cast<T2*>(&w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __hmax2(h[j], both<T2>(-INFINITY));  // (the operand that is a number)
+    return largest(w);
+  }
+  static __device__ __forceinline__ float largest(const uint4& w) {
+    const T2* h = reinterpret_cast<const T2*>(&w);
+    const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(to_f(m.x), to_f(m.y));
+  }
+};
+template <> struct Vec<__half> : Vec16<__half2> {};
+template <> struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat162> {};
 
 template <typename V, typename F>
 __device__ __forceinline__ V block_reduce(V v, F f, V* scratch) {
@@ -77,21 +146,34 @@ __device__ __forceinline__ V block_reduce(V v, F f, V* scratch) {
   if (lane == 0) scratch[warp] = v;
   __syncthreads();
   v = scratch[0];
+#pragma unroll
   for (int w = 1; w < kWarpsS; ++w) v = f(v, scratch[w]);
   return v;
 }
 
+__device__ __forceinline__ float exp2a(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int slice) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int slice) {
   extern __shared__ __align__(16) uint8_t sm[];
-  uint32_t* cnt = reinterpret_cast<uint32_t*>(sm);  // [kBins]
+  float* col = reinterpret_cast<float*>(sm);        // first split: [kSplit][kThreads]
+  uint32_t* cnt = reinterpret_cast<uint32_t*>(sm);  // histograms: [kBins] counts, masses (low and high half)
   uint32_t* mlo = cnt + kBins;
   uint32_t* mhi = mlo + kBins;
-  T* stage = reinterpret_cast<T*>(mhi + kBins);
-  __shared__ Red red[2];
-  __shared__ unsigned long long seg_s[2][2];   // this CTA's share of a round: count, mass
-  __shared__ unsigned long long found_s[2][4]; // the digit found: flag, digit, above, within
+  Token* all = reinterpret_cast<Token*>(sm);        // the first CTA's list of a row: [kCap] tokens,
+  unsigned long long* wall = reinterpret_cast<unsigned long long*>(all + kCap);  // and their weights
+  constexpr int kScratch = kSplit * kThreads * 4;   // the union of these
+  static_assert(3 * kBins * 4 <= kScratch && kCap * 16 <= kScratch, "scratch");
+  T* stage = reinterpret_cast<T*>(sm + kScratch);
+  __shared__ Red red;
+  __shared__ unsigned long long seg_s[2][2];    // histograms: this CTA's share
+  __shared__ unsigned long long found_s[2][4];  // the bin found: flag, bin, before it, its count
   __shared__ unsigned long long scratch[kWarpsS];
+  __shared__ int top_s;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
   const int row = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -99,33 +181,55 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int slic
   pdl_trigger();
   const int lo = min(a.vocab, rank * slice), n = min(a.vocab, lo + slice) - lo;
   const T* g = static_cast<const T*>(a.logits) + (size_t)row * a.logits_stride + lo;
-  // ---- the slice, kept at the same 16-byte phase as in global memory
+  // ---- the slice, padded to whole 16 bytes with tokens of -infinity.  A thread's elements (and so the order of
+  // every sum) do not depend on the row's address: a row that starts off a 16-byte boundary is shifted here.
   constexpr int VE = 16 / sizeof(T);
-  const int phase = (int)((reinterpret_cast<uintptr_t>(g) & 15) / sizeof(T));
-  T* x = stage + phase;
-  {
-    const int head = min(n, (VE - phase) % VE), body = (n - head) / VE;
-    for (int i = tid; i < head; i += kThreads) x[i] = g[i];
-    for (int i = tid; i < body; i += kThreads)
-      reinterpret_cast<uint4*>(x + head)[i] = ld_stream_u4(g + head + i * VE);
-    for (int i = head + body * VE + tid; i < n; i += kThreads) x[i] = g[i];
+  const int phase = (int)((reinterpret_cast<uintptr_t>(g) & 15) / sizeof(T)), nvec = (n + VE - 1) / VE;
+  float mine = -INFINITY;  // this thread's largest
+  if (!phase) {
+#pragma unroll 4
+    for (int i = tid; i < n / VE; i += kThreads) {
+      uint4 w = ld_stream_u4(g + i * VE);
+      mine = fmaxf(mine, Vec<T>::clean(w));
+      *reinterpret_cast<uint4*>(stage + i * VE) = w;
+    }
+  }
+#pragma unroll 1
+  for (int i = (phase ? 0 : n / VE * VE) + tid; i < nvec * VE; i += kThreads) {
+    const float f = i < n ? fmaxf(to_f<T>(g[i]), -INFINITY) : -INFINITY;
+    mine = fmaxf(mine, f);
+    stage[i] = from_f<T>(f);
   }
   __syncthreads();
-  float t = a.temperature ? __ldg(a.temperature + row) : 1.f;
+  // f(logit, index in the slice) for every element of a thread in 16 bytes whose largest is at least `least`
+  auto each = [&](float least, auto f) {
+#pragma unroll 1
+    for (int i = tid; i < nvec; i += kThreads) {
+      const uint4 w = *reinterpret_cast<const uint4*>(stage + i * VE);
+      if (Vec<T>::largest(w) < least) continue;
+      const T* v = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) f(to_f<T>(v[j]) + 0.f, i * VE + j);  // (-0 and 0 are one value)
+    }
+  };
+  const float t0 = a.temperature ? __ldg(a.temperature + row) : 1.f;
   int k = a.top_k ? __ldg(a.top_k + row) : 0;
   float tp = a.top_p ? __ldg(a.top_p + row) : 1.f;
-  const float mp = a.min_p ? __ldg(a.min_p + row) : 0.f;
-  if (!(t > 0.f)) t = 1.f, k = 1;
+  float mp = a.min_p ? fminf(__ldg(a.min_p + row), 1.f) : 0.f;
+  const bool greedy = !(t0 > 0.f);
+  const float t = greedy ? 1.f : t0;
+  if (greedy) k = 0, tp = 1.f, mp = 0.f;
   if (k <= 0 || k > a.vocab) k = a.vocab;
   const bool use_p = tp < 1.f;  // (false for NaN)
+  tp = fmaxf(tp, 0.f);
 
-  // ---- maximum and normaliser
-  float m = -INFINITY;
-  for (int i = tid; i < n; i += kThreads) m = fmaxf(m, logit(x, i));
-  m = block_reduce(m, [](float p, float q) { return fmaxf(p, q); }, reinterpret_cast<float*>(scratch));
-  if (tid == 0) red[0].maxv = m;
+  // ---- maximum
+  float m = block_reduce(mine, [](float p, float q) { return fmaxf(p, q); }, reinterpret_cast<float*>(scratch));
+  if (tid == 0) red.maxv = m;
+  for (int i = tid; i < kTop; i += kThreads) red.top[i] = 0;
   cluster.sync();
-  for (int r = 0; r < C; ++r) m = fmaxf(m, cluster.map_shared_rank(red, r)[0].maxv);
+  for (int r = 0; r < C; ++r) m = fmaxf(m, cluster.map_shared_rank(&red, r)->maxv);
+  m += 0.f;
   if (m == -INFINITY) {  // nothing to choose from
     if (rank == 0 && tid == 0) {
       a.tokens[row] = -1;
@@ -134,170 +238,401 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int slic
     cluster.sync();
     return;
   }
-  float z = 0.f;
-  for (int i = tid; i < n; i += kThreads) {
-    const float v = logit(x, i);
-    z += v == m ? 1.f : expf(v - m);  // (m may be infinite)
+  if (m == INFINITY) {  // the infinite logits share everything: zeros among tokens of -infinity
+    for (int i = tid; i < nvec * VE; i += kThreads) stage[i] = from_f<T>(to_f<T>(stage[i]) == m ? 0.f : -INFINITY);
+    mine = mine == m ? 0.f : -INFINITY;
+    m = 0.f;
+    __syncthreads();
   }
-  z = block_reduce(z, [](float p, float q) { return p + q; }, reinterpret_cast<float*>(scratch));
-  if (tid == 0) red[0].sum = z;
-
-  const float rt = 1.f / t;
-  auto weight = [&](float v) { return v == m ? 1.f : expf((v - m) * rt); };
-  constexpr int KB = sizeof(T) * 8;
-  const int ib = 32 - __clz(a.vocab - 1 > 0 ? a.vocab - 1 : 1);  // bits of an index
-  auto key_of = [&](int i, float v) {
-    return ((unsigned long long)ordered<T>(v) << ib) | (unsigned)(a.vocab - 1 - (lo + i));
+  const float c2 = 1.4426950408889634f / t;
+  auto weight = [&](float v) { return exp2a((v - m) * c2); };
+  if (a.logprobs) {
+    float z = 0.f;
+    each(-INFINITY, [&](float v, int) { z += exp2a((v - m) * 1.4426950408889634f); });
+    z = block_reduce(z, [](float p, float q) { return p + q; }, reinterpret_cast<float*>(scratch));
+    if (tid == 0) red.sum = z;
+  }
+  // the race's result; called by one thread of the first CTA, after a barrier that follows red.sum
+  auto finish = [&](unsigned long long best) {
+    const int token = (int)(0xffffffffu - (unsigned)(best & 0xffffffffu));
+    a.tokens[row] = token;
+    if (a.logprobs) {
+      float zs = 0.f;
+      for (int r = 0; r < C; ++r) zs += cluster.map_shared_rank(&red, r)->sum;
+      const float v = to_f<T>(static_cast<const T*>(a.logits)[(size_t)row * a.logits_stride + token]);
+      a.logprobs[row] = (v == INFINITY ? 0.f : v - m) - logf(zs);
+    }
   };
-  int round = 0;
-  // The composite key of the last token of the order such that `want` (tokens, or mass) is reached, among
-  // tokens with key >= floor_key.  `all`: what those hold together (want <= all).
-  auto descend = [&](bool by_mass, unsigned long long want, unsigned long long floor_key) {
-    unsigned long long prefix = 0, above = 0;  // key bits fixed so far; count or mass of larger prefixes
-    int left = KB + ib;                        // key bits not fixed yet
-    while (left > 0) {
-      const int d = min(kDigit, left), shift = left - d;
-      for (int b = tid; b < kBins; b += kThreads) cnt[b] = mlo[b] = mhi[b] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += kThreads) {
-        const float v = logit(x, i);
-        const unsigned long long key = key_of(i, v);
-        if (key < floor_key || (left < KB + ib && (key >> left) != prefix)) continue;
-        const int b = (int)((key >> shift) & ((1u << d) - 1));
-        atomicAdd(cnt + b, 1u);
-        if (by_mass) {
-          const unsigned long long f = fixed32(weight(v));
-          if (f) {
-            atomicAdd(mlo + b, (uint32_t)(f & 0xffffu));
-            atomicAdd(mhi + b, (uint32_t)(f >> 16));
-          }
-        }
+  const float* noise = a.noise + (size_t)row * a.noise_stride;
+  auto ticket = [&](float w, float e, int token) {  // larger for a larger w / e, then for a lower index
+    const float q = __fdiv_rn(w, e);
+    return ((unsigned long long)(q >= 0.f ? __float_as_uint(q) & 0x7fffffffu : 0u) << 32) |  // (bad noise never wins)
+           (0xffffffffu - (unsigned)token);
+  };
+  auto max64 = [](unsigned long long p, unsigned long long q) { return p > q ? p : q; };
+  auto add64 = [](unsigned long long p, unsigned long long q) { return p + q; };
+
+  Token cut{-INFINITY, a.vocab};  // tokens up to this one in the order are kept
+  // Collects the tokens that in(v) holds for in the CTAs' lists (all of them have values of `least` and more), and,
+  // where they fit, all of them in the first CTA's.  Returns their number.
+  auto collect = [&](float least, auto in) {
+    if (tid == 0) red.got = 0;
+    __syncthreads();
+    each(least, [&](float v, int i) {
+      if (!in(v) || before(cut, Token{v, lo + i})) return;
+      const int p = atomicAdd(&red.got, 1);
+      if (p < kCap) red.list[p] = Token{v, lo + i};
+    });
+    cluster.sync();
+    int got = 0;
+    for (int r = 0; r < C; ++r) {
+      const Red* o = cluster.map_shared_rank(&red, r);
+      const int c = o->got;
+      if (rank == 0 && got + c <= kCap)
+        for (int i = tid; i < c; i += kThreads) all[got + i] = o->list[i];
+      got += c;
+    }
+    __syncthreads();
+    return got;
+  };
+  // This thread's token of the first CTA's list, the number of tokens before it and their mass
+  Token me;
+  float wt;
+  int place;
+  unsigned long long ahead;
+  auto rank_all = [&](int got) {
+    me = tid < got ? all[tid] : Token{-INFINITY, a.vocab};
+    wt = tid < got ? weight(me.x) : 0.f;
+    if (tid < got) wall[tid] = fixed32(wt);
+    __syncthreads();
+    place = 0, ahead = 0;
+    if (tid < got) {
+#pragma unroll 4
+      for (int j = 0; j < got; ++j)
+        if (before(all[j], me)) ++place, ahead += wall[j];
+    }
+  };
+  // The rest of a row whose kept tokens are all in the list; `need`: the mass that top-p asks for, 0: the share
+  // of the first k tokens'
+  auto conclude = [&](int got, unsigned long long need) {
+    rank_all(got);
+    bool keep = tid < got && place < k;
+    if (use_p) {
+      if (!need) {
+        const unsigned long long kept = block_reduce(keep ? wall[tid] : 0ull, add64, scratch);
+        need = (unsigned long long)ceil((double)tp * (double)kept);
       }
-      cluster.sync();
-      // this CTA sums its share of the digits, the highest ones in rank 0: thread q the digits
-      // [top - q * per - per, top - q * per) of the share
-      const int share = kBins / C, per = (share + kThreads - 1) / kThreads;
-      const int hi_digit = kBins - rank * share;  // exclusive
-      unsigned long long tc[kBins / kThreads], tm[kBins / kThreads], c0 = 0, m0 = 0;
+      keep = keep && (ahead < need || place == 0);
+    }
+    keep = keep && wt >= mp;
+    const unsigned long long best = block_reduce(keep ? ticket(wt, __ldg(noise + me.index), me.index) : 0ull, max64, scratch);
+    if (tid == 0) finish(best);
+  };
+
+  // ---- top-k from the threads' maxima
+  if (k <= kCap && k < a.vocab) {
+    auto bin_of = [&](float v) { return (int)fminf((m - v) * 8.f, (float)(kTop - 1)); };
+    if (mine > -INFINITY) atomicAdd(&red.top[bin_of(mine)], 1);
+    cluster.sync();
+    if (warp == 0) {
+      int own[kTop / 32], sum = 0;
 #pragma unroll
-      for (int q = 0; q < kBins / kThreads; ++q) {
-        tc[q] = tm[q] = 0;
-        const int off = tid * per + q;
-        if (q < per && off < share) {
-          const int b = hi_digit - 1 - off;
-          for (int r = 0; r < C; ++r) {
-            tc[q] += cluster.map_shared_rank(cnt, r)[b];
-            if (by_mass)
-              tm[q] += ((unsigned long long)cluster.map_shared_rank(mhi, r)[b] << 16) + cluster.map_shared_rank(mlo, r)[b];
-          }
-          c0 += tc[q], m0 += tm[q];
-        }
+      for (int q = 0; q < kTop / 32; ++q) {
+        own[q] = 0;
+        for (int r = 0; r < C; ++r) own[q] += cluster.map_shared_rank(&red, r)->top[lane * (kTop / 32) + q];
+        sum += own[q];
       }
-      unsigned long long val = by_mass ? m0 : c0, inc = val;
+      int inc = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long u = __shfl_up_sync(0xffffffffu, inc, o);
+        const int u = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += u;
       }
-      __syncthreads();
-      if (lane == 31) scratch[warp] = inc;
-      __syncthreads();
-      unsigned long long before = inc - val, total = 0;
-      for (int w = 0; w < kWarpsS; ++w) {
-        if (w < warp) before += scratch[w];
-        total += scratch[w];
-      }
-      const int par = round & 1;
-      if (tid == 0) seg_s[par][0] = total, found_s[par][0] = 0;
-      cluster.sync();
-      for (int r = 0; r < rank; ++r) before += cluster.map_shared_rank(seg_s, r)[par][0];
-      before += above;
+      int at = kTop - 1, run = inc - sum;
 #pragma unroll
-      for (int q = 0; q < kBins / kThreads; ++q) {
-        const unsigned long long w = by_mass ? tm[q] : tc[q];
-        if (before < want && want <= before + w) {
-          for (int r = 0; r < C; ++r) {
-            auto* f = cluster.map_shared_rank(found_s, r)[par];
-            f[1] = (unsigned)(hi_digit - 1 - (tid * per + q));
-            f[2] = before;
-            f[3] = tc[q];
-            f[0] = 1 + (!by_mass && before + w == want ? 1 : 0);  // 2: the bucket is taken whole
-          }
-        }
-        before += w;
+      for (int q = kTop / 32 - 1; q >= 0; --q) {
+        int upto = run;
+#pragma unroll
+        for (int u = 0; u <= q; ++u) upto += own[u];
+        if (upto >= k) at = lane * (kTop / 32) + q;
       }
-      cluster.sync();
-      const unsigned long long flag = found_s[par][0], digit = found_s[par][1];
-      ++round;
-      above = found_s[par][2];
-      prefix = (prefix << d) | digit;
-      left = shift;
-      if (flag == 2) break;
-      if (flag == 0) return floor_key;                       // (cannot happen: want <= all)
-      if (found_s[par][3] == 1) break;                       // one token: it is the last one
+      at = __reduce_min_sync(0xffffffffu, at);
+      if (lane == 0) top_s = at;
     }
-    return max(prefix << left, floor_key);  // every token of the bucket is kept, or its only one
-  };
+    __syncthreads();
+    const int at = top_s;
+    if (at < kTop - 1) {
+      const int got = collect(m - (float)(at + 2) * 0.125f, [&](float v) { return bin_of(v) <= at; });
+      if (got <= kCap) {
+        if (rank == 0) conclude(got, 0);
+        cluster.sync();  // the others' shared memory stays until rank 0 has read it
+        return;
+      }
+      cluster.sync();  // (before the lists are used again)
+    }
+  }
 
-  unsigned long long cut = 0;
-  if (k < a.vocab) cut = descend(false, (unsigned long long)k, 0);
-  if (use_p) {
-    unsigned long long mass = 0;
-    for (int i = tid; i < n; i += kThreads) {
-      const float v = logit(x, i);
-      if (key_of(i, v) >= cut) mass += fixed32(weight(v));
-    }
-    mass = block_reduce(mass, [](unsigned long long p, unsigned long long q) { return p + q; }, scratch);
-    if (tid == 0) red[0].mass = mass;
+  // ---- the border, by count (top-k) and by mass (top-p)
+  int round = 0;
+  // After every CTA has filled its histogram: the bin, from the highest one down, with which `goal` is reached (or
+  // all there is, if that is less).  Leaves it in found_s of the round's parity.
+  auto find = [&](bool by_mass, unsigned long long goal) {
     cluster.sync();
-    mass = 0;
-    for (int r = 0; r < C; ++r) mass += cluster.map_shared_rank(red, r)[0].mass;
-    unsigned long long want = (unsigned long long)ceil((double)fmaxf(tp, 0.f) * (double)mass);
-    want = min(max(want, 1ull), mass);
-    cut = descend(true, want, cut);
+    // this CTA sums its share of the bins, the highest ones in rank 0, `per` of them a thread
+    const int share = kBins / C, per = (share + kThreads - 1) / kThreads;
+    const int hi_bin = kBins - rank * share;  // exclusive
+    unsigned long long tc[kBins / kThreads], tm[kBins / kThreads], val = 0;
+#pragma unroll
+    for (int q = 0; q < kBins / kThreads; ++q) {
+      tc[q] = tm[q] = 0;
+      const int off = tid * per + q;
+      if (q < per && off < share) {
+        const int b = hi_bin - 1 - off;
+        for (int r = 0; r < C; ++r) {
+          tc[q] += cluster.map_shared_rank(cnt, r)[b];
+          if (by_mass)
+            tm[q] += ((unsigned long long)cluster.map_shared_rank(mhi, r)[b] << 16) + cluster.map_shared_rank(mlo, r)[b];
+        }
+        val += by_mass ? tm[q] : tc[q];
+      }
+    }
+    unsigned long long inc = val;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    __syncthreads();
+    if (lane == 31) scratch[warp] = inc;
+    __syncthreads();
+    unsigned long long ahead_ = inc - val, total = 0;
+    for (int w = 0; w < kWarpsS; ++w) {
+      if (w < warp) ahead_ += scratch[w];
+      total += scratch[w];
+    }
+    const int par = round++ & 1;
+    if (tid == 0) seg_s[par][0] = total, found_s[par][0] = 0;
+    cluster.sync();
+    unsigned long long sum = 0;
+    for (int r = 0; r < C; ++r) {
+      if (r < rank) ahead_ += cluster.map_shared_rank(seg_s, r)[par][0];
+      sum += cluster.map_shared_rank(seg_s, r)[par][0];
+    }
+    goal = min(goal, sum);
+#pragma unroll
+    for (int q = 0; q < kBins / kThreads; ++q) {
+      const unsigned long long w = by_mass ? tm[q] : tc[q];
+      if (ahead_ < goal && goal <= ahead_ + w) {
+        for (int r = 0; r < C; ++r) {
+          auto* f = cluster.map_shared_rank(found_s, r)[par];
+          f[1] = (unsigned)(hi_bin - 1 - (tid * per + q));
+          f[2] = ahead_;
+          f[3] = tc[q];
+          f[0] = 1 + (!by_mass && ahead_ + w == goal ? 1 : 0);  // 2: the bin is taken whole
+        }
+      }
+      ahead_ += w;
+    }
+    cluster.sync();
+    return par;
+  };
+  auto clear = [&]() {
+    for (int b = tid; b < 3 * kBins; b += kThreads) cnt[b] = 0;
+    __syncthreads();
+  };
+  auto count_in = [&](int b, bool by_mass, float v) {
+    atomicAdd(cnt + b, 1u);
+    if (by_mass) {
+      const unsigned long long f = fixed32(weight(v));
+      if (f) {
+        atomicAdd(mlo + b, (uint32_t)(f & 0xffffu));
+        atomicAdd(mhi + b, (uint32_t)(f >> 16));
+      }
+    }
+  };
+#pragma unroll 1
+  for (int by_mass = 0; by_mass < 2; ++by_mass) {
+    if (by_mass ? !use_p : k >= a.vocab) continue;
+    // ---- 16 bins of d = m - v, the last one without an end
+    const float w = by_mass ? fminf(fmaxf(1.0397208f * t, 1e-3f), 64.f) : 1.f, rw = 1.f / w;
+    constexpr float kMagic = 8388608.f;  // + 2^23 rounds to a whole number, in the low bits
+    auto bin_of = [&](float v) { return __float_as_uint(fminf((m - v) * rw, (float)(kSplit - 1)) + kMagic) & 31u; };
+#pragma unroll
+    for (int b = 0; b < kSplit; ++b) col[b * kThreads + tid] = 0.f;
+    each(-INFINITY, [&](float v, int i) {
+      if (v == -INFINITY || before(cut, Token{v, lo + i})) return;
+      col[bin_of(v) * kThreads + tid] += by_mass ? weight(v) : 1.f;
+    });
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int q = 0; q < kThreads / 32; ++q) s += col[warp * kThreads + q * 32 + lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) red.bin[by_mass][warp] = s;
+    cluster.sync();
+    float sum[kSplit], total = 0.f;
+#pragma unroll
+    for (int b = 0; b < kSplit; ++b) sum[b] = 0.f;
+#pragma unroll 1
+    for (int r = 0; r < C; ++r) {
+      const Red* o = cluster.map_shared_rank(&red, r);
+#pragma unroll
+      for (int b = 0; b < kSplit; ++b) sum[b] += o->bin[by_mass][b];
+    }
+#pragma unroll
+    for (int b = 0; b < kSplit; ++b) total += sum[b];
+    if (!by_mass && total <= (float)k) continue;  // (tokens of -infinity are never kept)
+    const float want = by_mass ? tp * total : (float)k;
+    float above = 0.f, upto = 0.f, few = 0.f;
+    int at = -1;
+#pragma unroll
+    for (int b = 0; b < kSplit; ++b)
+      if (at < 0) {
+        above = upto;
+        upto += sum[b];
+        // at least so many tokens: none of the bin's weighs more than its first
+        few += !by_mass ? sum[b] : sum[b] > 0.f ? sum[b] / exp2a(-fmaxf((float)b - 0.5f, 0.f) * w * c2) : 0.f;
+        if (upto >= want || b == kSplit - 1) at = b;
+      }
+    const float rest = want - above;
+    const unsigned long long need = by_mass ? (unsigned long long)((double)want * 4294967296.0) : 0;
+    const float least = at == kSplit - 1 ? -INFINITY : m - ((float)at + 0.501f) * w;  // no token of the bins is smaller
+    int got = kCap + 1;
+    bool whole = few <= (float)kCap;
+    if (whole) {
+      got = collect(least, [&](float v) { return v > -INFINITY && (int)bin_of(v) <= at; });
+      if (got > kCap) cluster.sync();  // (before the lists are used again)
+    }
+    if (got > kCap) {
+      // ---- the tokens of that bin in 2048, the largest ones in the highest
+      whole = false;
+      const float from = fmaxf((float)at - 0.5f, 0.f);
+      auto fine = [&](float v) {
+        const float h = fmaxf((m - v) * rw - from, 0.f);
+        // (the last bin has no end: a rising function of it that does)
+        const float q = at == kSplit - 1 ? 1.f - __fdiv_rn(16.f, h + 16.f) : h;
+        return kBins - 1 - (int)fminf(q * (float)kBins, (float)(kBins - 1));
+      };
+      clear();
+      each(least, [&](float v, int i) {
+        if (v == -INFINITY || (int)bin_of(v) != at || before(cut, Token{v, lo + i})) return;
+        count_in(fine(v), by_mass, v);
+      });
+      const int par = find(by_mass, max(1ull, by_mass ? (unsigned long long)((double)rest * 4294967296.0)
+                                                      : (unsigned long long)rest));
+      const int bin = (int)found_s[par][1];
+      const unsigned long long over = found_s[par][2];
+      if (found_s[par][0] && found_s[par][3] <= kCap) {
+        got = collect(least, [&](float v) { return v > -INFINITY && (int)bin_of(v) == at && fine(v) == bin; });
+        if (rank == 0) {
+          rank_all(got);
+          const double goal = by_mass ? (double)rest * 4294967296.0 - (double)over : (double)rest - (double)over;
+          const int last = max(1, __syncthreads_count(tid < got && (by_mass ? (double)ahead : (double)place) < goal)) - 1;
+          if (tid < got && place == last)
+            for (int r = 0; r < C; ++r) cluster.map_shared_rank(&red, r)->cut = me;
+        }
+        cluster.sync();
+        cut = red.cut;
+        continue;
+      }
+    } else {
+      if (rank == 0) conclude(got, by_mass ? max(need, 1ull) : 0);
+      cluster.sync();
+      return;
+    }
+    // ---- crowded: radix descent to the last token such that `goal` tokens, or that much mass, is reached
+    constexpr int KB = sizeof(T) * 8;
+    const int ib = 32 - __clz(a.vocab - 1 > 0 ? a.vocab - 1 : 1);  // bits of an index
+    unsigned long long prefix = 0, over = 0;  // key bits fixed so far; count or mass of larger prefixes
+    unsigned long long goal = (unsigned long long)k;
+    if (by_mass) {
+      unsigned long long mass = 0;
+      each(-INFINITY, [&](float v, int i) {
+        if (v > -INFINITY && !before(cut, Token{v, lo + i})) mass += fixed32(weight(v));
+      });
+      mass = block_reduce(mass, add64, scratch);
+      if (tid == 0) red.mass = mass;
+      cluster.sync();
+      mass = 0;
+      for (int r = 0; r < C; ++r) mass += cluster.map_shared_rank(&red, r)->mass;
+      goal = min(max((unsigned long long)ceil((double)tp * (double)mass), 1ull), mass);
+    }
+    int left = KB + ib;  // key bits not fixed yet
+    while (left > 0) {
+      const int d = min(kDigit, left), shift = left - d;
+      clear();
+      each(-INFINITY, [&](float v, int i) {
+        if (i >= n || before(cut, Token{v, lo + i})) return;
+        const unsigned long long key = ((unsigned long long)ordered<T>(v) << ib) | (unsigned)(a.vocab - 1 - (lo + i));
+        if (left < KB + ib && (key >> left) != prefix) return;
+        count_in((int)((key >> shift) & ((1u << d) - 1)), by_mass, v);
+      });
+      const int par = find(by_mass, goal - over);
+      over += found_s[par][2];
+      prefix = (prefix << d) | found_s[par][1];
+      left = shift;
+      // taken whole, or its one token is the last: all with keys from prefix << left on
+      if (found_s[par][0] != 1 || found_s[par][3] == 1) break;
+    }
+    const unsigned long long bound = prefix << left;
+    const Token b{from_ordered<T>((uint32_t)(bound >> ib)), a.vocab - 1 - (int)(bound & ((1ull << ib) - 1))};
+    if (before(b, cut)) cut = b;
   }
 
   // ---- the race
-  const float* e = a.noise + (size_t)row * a.noise_stride + lo;
   unsigned long long best = 0;
-  for (int i = tid; i < n; i += kThreads) {
-    const float v = logit(x, i);
-    if (v == -INFINITY || key_of(i, v) < cut) continue;
-    const float w = weight(v);
-    if (mp > 0.f && w < fminf(mp, 1.f)) continue;
-    const float q = __fdiv_rn(w, __ldg(e + i));
-    const uint32_t bits = q >= 0.f ? __float_as_uint(q) : 0u;  // (noise that is negative or NaN never wins)
-    const unsigned long long cand = ((unsigned long long)(bits & 0x7fffffffu) << 32) | (0xffffffffu - (unsigned)(lo + i));
-    best = max(best, cand);
+  if (greedy) {
+    each(m, [&](float v, int i) {
+      if (v == m) best = max64(best, (1ull << 32) | (0xffffffffu - (unsigned)(lo + i)));
+    });
+  } else {
+    // min-p as a bound of the logit (a little low: the weight itself decides)
+    const float least = fmaxf(cut.x, mp > 0.f ? m + (log2f(mp) * 1.0001f - 1e-3f) / c2 : -INFINITY);
+    const float* e = noise + lo;
+    const bool vec = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
+    float lead = -1.f;  // a little below the best quotient so far
+#pragma unroll 1
+    for (int i = tid; i < nvec; i += kThreads) {
+      const uint4 w = *reinterpret_cast<const uint4*>(stage + i * VE);
+      if (Vec<T>::largest(w) < least) continue;
+      const T* v = reinterpret_cast<const T*>(&w);
+      float en[VE];
+      const bool wide = vec && least == -INFINITY && (i + 1) * VE <= n;  // all tokens are kept
+      if (wide)
+#pragma unroll
+        for (int q = 0; q < VE / 4; ++q)
+          *reinterpret_cast<uint4*>(en + 4 * q) = ld_stream_u4(e + i * VE + 4 * q);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        const float x = to_f<T>(v[j]) + 0.f;
+        const int at = i * VE + j;
+        if (x < least || x == -INFINITY || before(cut, Token{x, lo + at})) continue;
+        const float wt_ = weight(x), ej = wide ? en[j] : __ldg(e + at);
+        if (wt_ < mp || (wt_ <= lead * ej && ej > 0.f)) continue;  // (behind)
+        const unsigned long long cand = ticket(wt_, ej, lo + at);
+        if (cand > best) best = cand, lead = __uint_as_float((uint32_t)(cand >> 32)) * 0.999999f;
+      }
+    }
   }
-  best = block_reduce(best, [](unsigned long long p, unsigned long long q) { return p > q ? p : q; }, scratch);
-  if (tid == 0) red[0].best = best;
+  best = block_reduce(best, max64, scratch);
+  if (tid == 0) red.best = best;
   cluster.sync();
   if (rank == 0 && tid == 0) {
-    float zs = 0.f;
-    for (int r = 0; r < C; ++r) {
-      const Red* o = cluster.map_shared_rank(red, r);
-      best = max(best, o->best);
-      zs += o->sum;
-    }
-    const unsigned token = 0xffffffffu - (unsigned)(best & 0xffffffffu);
-    a.tokens[row] = token;
-    if (a.logprobs) {
-      const float v = logit(static_cast<const T*>(a.logits) + (size_t)row * a.logits_stride, (int)token);
-      a.logprobs[row] = (v == m ? 0.f : v - m) - logf(zs);
-    }
+    for (int r = 0; r < C; ++r) best = max64(best, cluster.map_shared_rank(&red, r)->best);
+    finish(best);
   }
   cluster.sync();  // the others' shared memory stays until rank 0 has read it
 }
 
 template <typename T>
 cudaError_t launch_t(const SampleArgs& a, cudaStream_t st) {
-  // CTAs of a row: enough that a slice fits in 64 KB (three CTAs an SM), and as many as keep one wave
+  // CTAs of a row: enough that a slice fits in 64 KB (two CTAs an SM), more while all rows fit in one wave
   int C = 1;
   while (C < kMaxCluster && ((int64_t)a.vocab * (int64_t)sizeof(T) > C * 65536ll || (int64_t)a.rows * C * 2 <= num_sms()))
     C *= 2;
   const int slice = (div_up(a.vocab, C) + 7) / 8 * 8;
-  const size_t smem = 3 * kBins * sizeof(uint32_t) + (size_t)slice * sizeof(T) + 16;
+  const size_t smem = kSplit * kThreads * 4 + (size_t)slice * sizeof(T) + 16;
   auto kern = sample_kernel<T>;
   if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
   cudaLaunchConfig_t cfg{};
