@@ -17,11 +17,11 @@
 //     kCap), which finishes the row alone: the rank and the mass before each token by comparison with every
 //     other, then top-k, top-p, min-p and the race.
 //   * top-p (and a top-k too large for that): tokens are split by d = M - x into 16 bins, then those of the bin
-//     that holds the border into 2048.  In the first split every thread adds its elements to bins of its own (a
+//     that holds the border into 512.  In the first split every thread adds its elements to bins of its own (a
 //     column of shared memory): no atomics, and fp32 sums that always add in the same order.  The tokens of the
 //     last bin, or all up to it where those are few, go to the first CTA, which finds the border; all CTAs race.
 //   * Rows that stay crowded (hundreds of equal logits at the border) go through radix descent over the composite
-//     key (logit as an ordered integer, inverted index), 11 bits a round, with integer atomics.
+//     key (logit as an ordered integer, inverted index), 9 bits a round, with integer atomics.
 //   * Masses of single tokens are summed as fixed-point integers (w 2^32 rounded, at most 2^-33 of the largest
 //     weight off per token), so no sum depends on the order of atomics: equal inputs give equal tokens.
 #include <cooperative_groups.h>
@@ -38,13 +38,14 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarpsS = kThreads / 32;
-constexpr int kDigit = 11, kBins = 1 << kDigit;
+constexpr int kDigit = 9, kBins = 1 << kDigit;  // a thread sums one bin at most
 constexpr int kMaxCluster = 8;
 
 constexpr int kSplit = 16;   // bins of the first split: one warp adds up each
 constexpr int kCap = kThreads;  // tokens that one CTA finishes alone, one per thread
 constexpr int kTop = 128;    // bins of the threads' maxima
-static_assert(kSplit == kWarpsS && kCap <= kThreads, "one warp a bin, one thread a token");
+constexpr int kNear = 1024;  // tokens of the border's bin that a warp lists
+static_assert(kSplit == kWarpsS && kCap <= kThreads && kBins <= kThreads, "one warp a bin, one thread a token");
 
 struct Token {
   float x;
@@ -161,19 +162,21 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int slice) {
   extern __shared__ __align__(16) uint8_t sm[];
   float* col = reinterpret_cast<float*>(sm);        // first split: [kSplit][kThreads]
-  uint32_t* cnt = reinterpret_cast<uint32_t*>(sm);  // histograms: [kBins] counts, masses (low and high half)
-  uint32_t* mlo = cnt + kBins;
-  uint32_t* mhi = mlo + kBins;
+  uint16_t* near = reinterpret_cast<uint16_t*>(sm) + (threadIdx.x >> 5) * kNear;  // a warp's tokens of one bin
   Token* all = reinterpret_cast<Token*>(sm);        // the first CTA's list of a row: [kCap] tokens,
   unsigned long long* wall = reinterpret_cast<unsigned long long*>(all + kCap);  // and their weights
   constexpr int kScratch = kSplit * kThreads * 4;   // the union of these
-  static_assert(3 * kBins * 4 <= kScratch && kCap * 16 <= kScratch, "scratch");
-  T* stage = reinterpret_cast<T*>(sm + kScratch);
+  static_assert(kWarpsS * kNear * 2 <= kScratch && kCap * 16 <= kScratch, "scratch");
+  uint32_t* cnt = reinterpret_cast<uint32_t*>(sm + kScratch);  // histograms: [kBins] counts, masses (low, high half)
+  uint32_t* mlo = cnt + kBins;
+  uint32_t* mhi = mlo + kBins;
+  T* stage = reinterpret_cast<T*>(mhi + kBins);
   __shared__ Red red;
   __shared__ unsigned long long seg_s[2][2];    // histograms: this CTA's share
   __shared__ unsigned long long found_s[2][4];  // the bin found: flag, bin, before it, its count
   __shared__ unsigned long long scratch[kWarpsS];
-  __shared__ int top_s;
+  __shared__ int top_s, lead_s;
+  __shared__ unsigned long long best_s;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
   const int row = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -228,7 +231,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   if (tid == 0) red.maxv = m;
   for (int i = tid; i < kTop; i += kThreads) red.top[i] = 0;
   cluster.sync();
-  for (int r = 0; r < C; ++r) m = fmaxf(m, cluster.map_shared_rank(&red, r)->maxv);
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; ++r)
+    if (r < C) m = fmaxf(m, cluster.map_shared_rank(&red, r)->maxv);
   m += 0.f;
   if (m == -INFINITY) {  // nothing to choose from
     if (rank == 0 && tid == 0) {
@@ -258,7 +263,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     a.tokens[row] = token;
     if (a.logprobs) {
       float zs = 0.f;
-      for (int r = 0; r < C; ++r) zs += cluster.map_shared_rank(&red, r)->sum;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < C) zs += cluster.map_shared_rank(&red, r)->sum;
       const float v = to_f<T>(static_cast<const T*>(a.logits)[(size_t)row * a.logits_stride + token]);
       a.logprobs[row] = (v == INFINITY ? 0.f : v - m) - logf(zs);
     }
@@ -273,16 +280,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   auto add64 = [](unsigned long long p, unsigned long long q) { return p + q; };
 
   Token cut{-INFINITY, a.vocab};  // tokens up to this one in the order are kept
-  // Collects the tokens that in(v) holds for in the CTAs' lists (all of them have values of `least` and more), and,
-  // where they fit, all of them in the first CTA's.  Returns their number.
-  auto collect = [&](float least, auto in) {
-    if (tid == 0) red.got = 0;
-    __syncthreads();
-    each(least, [&](float v, int i) {
-      if (!in(v) || before(cut, Token{v, lo + i})) return;
-      const int p = atomicAdd(&red.got, 1);
-      if (p < kCap) red.list[p] = Token{v, lo + i};
-    });
+  auto put = [&](float v, int i) {
+    const int p = atomicAdd(&red.got, 1);
+    if (p < kCap) red.list[p] = Token{v, lo + i};
+  };
+  auto gather = [&]() {  // the CTAs' lists, where they fit, into the first CTA's; the number of their tokens
     cluster.sync();
     int got = 0;
     for (int r = 0; r < C; ++r) {
@@ -294,6 +296,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     }
     __syncthreads();
     return got;
+  };
+  // Collects the tokens that in(v) holds for in the CTAs' lists (all of them have values of `least` and more), and,
+  // where they fit, all of them in the first CTA's.  Returns their number.
+  auto collect = [&](float least, auto in) {
+    if (tid == 0) red.got = 0;
+    __syncthreads();
+    each(least, [&](float v, int i) {
+      if (in(v)) put(v, i);
+    });
+    return gather();
   };
   // This thread's token of the first CTA's list, the number of tokens before it and their mass
   Token me;
@@ -339,7 +351,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
 #pragma unroll
       for (int q = 0; q < kTop / 32; ++q) {
         own[q] = 0;
-        for (int r = 0; r < C; ++r) own[q] += cluster.map_shared_rank(&red, r)->top[lane * (kTop / 32) + q];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r)
+          if (r < C) own[q] += cluster.map_shared_rank(&red, r)->top[lane * (kTop / 32) + q];
         sum += own[q];
       }
       int inc = sum;
@@ -378,23 +392,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   // all there is, if that is less).  Leaves it in found_s of the round's parity.
   auto find = [&](bool by_mass, unsigned long long goal) {
     cluster.sync();
-    // this CTA sums its share of the bins, the highest ones in rank 0, `per` of them a thread
-    const int share = kBins / C, per = (share + kThreads - 1) / kThreads;
-    const int hi_bin = kBins - rank * share;  // exclusive
-    unsigned long long tc[kBins / kThreads], tm[kBins / kThreads], val = 0;
+    // this CTA sums its share of the bins, the highest ones in rank 0, one a thread
+    const int share = kBins / C, bin = kBins - 1 - rank * share - tid;
+    unsigned long long own = 0, val = 0;
+    if (tid < share) {
 #pragma unroll
-    for (int q = 0; q < kBins / kThreads; ++q) {
-      tc[q] = tm[q] = 0;
-      const int off = tid * per + q;
-      if (q < per && off < share) {
-        const int b = hi_bin - 1 - off;
-        for (int r = 0; r < C; ++r) {
-          tc[q] += cluster.map_shared_rank(cnt, r)[b];
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < C) {
+          own += cluster.map_shared_rank(cnt, r)[bin];
           if (by_mass)
-            tm[q] += ((unsigned long long)cluster.map_shared_rank(mhi, r)[b] << 16) + cluster.map_shared_rank(mlo, r)[b];
+            val += ((unsigned long long)cluster.map_shared_rank(mhi, r)[bin] << 16) + cluster.map_shared_rank(mlo, r)[bin];
         }
-        val += by_mass ? tm[q] : tc[q];
-      }
+      if (!by_mass) val = own;
     }
     unsigned long long inc = val;
 #pragma unroll
@@ -414,27 +423,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     if (tid == 0) seg_s[par][0] = total, found_s[par][0] = 0;
     cluster.sync();
     unsigned long long sum = 0;
-    for (int r = 0; r < C; ++r) {
-      if (r < rank) ahead_ += cluster.map_shared_rank(seg_s, r)[par][0];
-      sum += cluster.map_shared_rank(seg_s, r)[par][0];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      const unsigned long long v = r < C ? cluster.map_shared_rank(seg_s, r)[par][0] : 0;
+      if (r < rank) ahead_ += v;
+      sum += v;
     }
     goal = min(goal, sum);
-#pragma unroll
-    for (int q = 0; q < kBins / kThreads; ++q) {
-      const unsigned long long w = by_mass ? tm[q] : tc[q];
-      if (ahead_ < goal && goal <= ahead_ + w) {
-        for (int r = 0; r < C; ++r) {
-          auto* f = cluster.map_shared_rank(found_s, r)[par];
-          f[1] = (unsigned)(hi_bin - 1 - (tid * per + q));
-          f[2] = ahead_;
-          f[3] = tc[q];
-          f[0] = 1 + (!by_mass && ahead_ + w == goal ? 1 : 0);  // 2: the bin is taken whole
-        }
+    if (ahead_ < goal && goal <= ahead_ + val)
+      for (int r = 0; r < C; ++r) {
+        auto* f = cluster.map_shared_rank(found_s, r)[par];
+        f[1] = (unsigned)bin;
+        f[2] = ahead_;
+        f[3] = own;
+        f[0] = 1 + (!by_mass && ahead_ + val == goal ? 1 : 0);  // 2: the bin is taken whole
       }
-      ahead_ += w;
-    }
     cluster.sync();
     return par;
+  };
+  auto erase = [&]() {  // what lies behind `cut` leaves the slice
+    each(-INFINITY, [&](float v, int i) {
+      if (before(cut, Token{v, lo + i})) stage[i] = from_f<T>(-INFINITY);
+    });
+    __syncthreads();
   };
   auto clear = [&]() {
     for (int b = tid; b < 3 * kBins; b += kThreads) cnt[b] = 0;
@@ -459,10 +470,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     auto bin_of = [&](float v) { return __float_as_uint(fminf((m - v) * rw, (float)(kSplit - 1)) + kMagic) & 31u; };
 #pragma unroll
     for (int b = 0; b < kSplit; ++b) col[b * kThreads + tid] = 0.f;
-    each(-INFINITY, [&](float v, int i) {
-      if (v == -INFINITY || before(cut, Token{v, lo + i})) return;
-      col[bin_of(v) * kThreads + tid] += by_mass ? weight(v) : 1.f;
-    });
+    if (by_mass)
+      each(-INFINITY, [&](float v, int) { col[bin_of(v) * kThreads + tid] += weight(v); });
+    else
+      each(-INFINITY, [&](float v, int) { col[bin_of(v) * kThreads + tid] += v > -INFINITY ? 1.f : 0.f; });
     __syncthreads();
     float s = 0.f;
 #pragma unroll
@@ -471,41 +482,39 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) red.bin[by_mass][warp] = s;
     cluster.sync();
-    float sum[kSplit], total = 0.f;
+    // every warp: one lane a bin, the same order of additions everywhere
+    float upto = 0.f, above, total, want;
+    int at;
+    bool whole;
+    {
 #pragma unroll
-    for (int b = 0; b < kSplit; ++b) sum[b] = 0.f;
-#pragma unroll 1
-    for (int r = 0; r < C; ++r) {
-      const Red* o = cluster.map_shared_rank(&red, r);
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < C) upto += cluster.map_shared_rank(&red, r)->bin[by_mass][lane & (kSplit - 1)];
+      // at least so many tokens are in the bin: none of them weighs more than its first
+      float few = !by_mass || upto == 0.f ? upto : upto / exp2a(-fmaxf((float)(lane & (kSplit - 1)) - 0.5f, 0.f) * w * c2);
 #pragma unroll
-      for (int b = 0; b < kSplit; ++b) sum[b] += o->bin[by_mass][b];
-    }
-#pragma unroll
-    for (int b = 0; b < kSplit; ++b) total += sum[b];
-    if (!by_mass && total <= (float)k) continue;  // (tokens of -infinity are never kept)
-    const float want = by_mass ? tp * total : (float)k;
-    float above = 0.f, upto = 0.f, few = 0.f;
-    int at = -1;
-#pragma unroll
-    for (int b = 0; b < kSplit; ++b)
-      if (at < 0) {
-        above = upto;
-        upto += sum[b];
-        // at least so many tokens: none of the bin's weighs more than its first
-        few += !by_mass ? sum[b] : sum[b] > 0.f ? sum[b] / exp2a(-fmaxf((float)b - 0.5f, 0.f) * w * c2) : 0.f;
-        if (upto >= want || b == kSplit - 1) at = b;
+      for (int o = 1; o < kSplit; o <<= 1) {
+        const float u = __shfl_up_sync(0xffffffffu, upto, o, kSplit), f = __shfl_up_sync(0xffffffffu, few, o, kSplit);
+        if ((lane & (kSplit - 1)) >= o) upto += u, few += f;
       }
+      total = __shfl_sync(0xffffffffu, upto, kSplit - 1);
+      want = by_mass ? tp * total : (float)k;
+      at = __ffs((int)(__ballot_sync(0xffffffffu, upto >= want) | 1u << (kSplit - 1))) - 1;
+      above = __shfl_sync(0xffffffffu, upto, max(at - 1, 0));
+      if (at == 0) above = 0.f;
+      whole = __shfl_sync(0xffffffffu, few, at) <= (float)kCap;
+    }
+    if (!by_mass && total <= (float)k) continue;  // (tokens of -infinity are never kept)
     const float rest = want - above;
     const unsigned long long need = by_mass ? (unsigned long long)((double)want * 4294967296.0) : 0;
     const float least = at == kSplit - 1 ? -INFINITY : m - ((float)at + 0.501f) * w;  // no token of the bins is smaller
     int got = kCap + 1;
-    bool whole = few <= (float)kCap;
     if (whole) {
       got = collect(least, [&](float v) { return v > -INFINITY && (int)bin_of(v) <= at; });
       if (got > kCap) cluster.sync();  // (before the lists are used again)
     }
     if (got > kCap) {
-      // ---- the tokens of that bin in 2048, the largest ones in the highest
+      // ---- the tokens of that bin in 512, the largest ones in the highest
       whole = false;
       const float from = fmaxf((float)at - 0.5f, 0.f);
       auto fine = [&](float v) {
@@ -514,17 +523,46 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
         const float q = at == kSplit - 1 ? 1.f - __fdiv_rn(16.f, h + 16.f) : h;
         return kBins - 1 - (int)fminf(q * (float)kBins, (float)(kBins - 1));
       };
+      // each warp lists its tokens of the bin (indices within the slice), then works on them with all lanes
+      int mine_n = 0;
+#pragma unroll 1
+      for (int i0 = warp * 32; i0 < nvec; i0 += kThreads) {
+        const int i = i0 + lane;
+        const uint4 w4 = i < nvec ? *reinterpret_cast<const uint4*>(stage + i * VE) : uint4{};
+        const T* v = reinterpret_cast<const T*>(&w4);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+          const float x = to_f<T>(v[j]);
+          const bool in = i < nvec && x > -INFINITY && (int)bin_of(x) == at;
+          const uint32_t mask = __ballot_sync(0xffffffffu, in);
+          const int to = mine_n + __popc(mask & ((1u << lane) - 1u));
+          if (in && to < kNear) near[to] = (uint16_t)(i * VE + j);
+          mine_n += __popc(mask);
+        }
+      }
       clear();
-      each(least, [&](float v, int i) {
-        if (v == -INFINITY || (int)bin_of(v) != at || before(cut, Token{v, lo + i})) return;
-        count_in(fine(v), by_mass, v);
-      });
+      auto visit = [&](auto f) {
+        if (mine_n <= kNear) {
+#pragma unroll 1
+          for (int q = lane; q < mine_n; q += 32) f(to_f<T>(stage[near[q]]) + 0.f, (int)near[q]);
+        } else {  // too many: from the slice (a warp's vectors are the ones it listed)
+          each(least, [&](float v, int i) {
+            if (v > -INFINITY && (int)bin_of(v) == at) f(v, i);
+          });
+        }
+      };
+      visit([&](float v, int) { count_in(fine(v), by_mass, v); });
       const int par = find(by_mass, max(1ull, by_mass ? (unsigned long long)((double)rest * 4294967296.0)
                                                       : (unsigned long long)rest));
       const int bin = (int)found_s[par][1];
       const unsigned long long over = found_s[par][2];
       if (found_s[par][0] && found_s[par][3] <= kCap) {
-        got = collect(least, [&](float v) { return v > -INFINITY && (int)bin_of(v) == at && fine(v) == bin; });
+        if (tid == 0) red.got = 0;
+        __syncthreads();
+        visit([&](float v, int i) {
+          if (fine(v) == bin) put(v, i);
+        });
+        got = gather();
         if (rank == 0) {
           rank_all(got);
           const double goal = by_mass ? (double)rest * 4294967296.0 - (double)over : (double)rest - (double)over;
@@ -534,6 +572,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
         }
         cluster.sync();
         cut = red.cut;
+        if (!by_mass && use_p) erase();
         continue;
       }
     } else {
@@ -549,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     if (by_mass) {
       unsigned long long mass = 0;
       each(-INFINITY, [&](float v, int i) {
-        if (v > -INFINITY && !before(cut, Token{v, lo + i})) mass += fixed32(weight(v));
+        if (v > -INFINITY) mass += fixed32(weight(v));
       });
       mass = block_reduce(mass, add64, scratch);
       if (tid == 0) red.mass = mass;
@@ -563,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       const int d = min(kDigit, left), shift = left - d;
       clear();
       each(-INFINITY, [&](float v, int i) {
-        if (i >= n || before(cut, Token{v, lo + i})) return;
+        if (i >= n) return;
         const unsigned long long key = ((unsigned long long)ordered<T>(v) << ib) | (unsigned)(a.vocab - 1 - (lo + i));
         if (left < KB + ib && (key >> left) != prefix) return;
         count_in((int)((key >> shift) & ((1u << d) - 1)), by_mass, v);
@@ -578,50 +617,72 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     const unsigned long long bound = prefix << left;
     const Token b{from_ordered<T>((uint32_t)(bound >> ib)), a.vocab - 1 - (int)(bound & ((1ull << ib) - 1))};
     if (before(b, cut)) cut = b;
+    if (!by_mass && use_p) erase();
   }
 
   // ---- the race
   unsigned long long best = 0;
+  // min-p as a bound of the logit (a little low: the weight itself decides)
+  const float least = greedy ? m : fmaxf(cut.x, mp > 0.f ? m + (log2f(mp) * 1.0001f - 1e-3f) / c2 : -INFINITY);
+  auto kept = [&](float v, int i) { return v > -INFINITY && !before(cut, Token{v, lo + i}) && weight(v) >= mp; };
   if (greedy) {
     each(m, [&](float v, int i) {
       if (v == m) best = max64(best, (1ull << 32) | (0xffffffffu - (unsigned)(lo + i)));
     });
   } else {
-    // min-p as a bound of the logit (a little low: the weight itself decides)
-    const float least = fmaxf(cut.x, mp > 0.f ? m + (log2f(mp) * 1.0001f - 1e-3f) / c2 : -INFINITY);
+    // All threads share the best quotient so far, a little lowered (lead_s): few tokens come near it, so the
+    // division that decides, and the tests of what is kept, run for those only.
+    if (tid == 0) best_s = 0, lead_s = 0;
+    __syncthreads();
     const float* e = noise + lo;
     const bool vec = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
-    float lead = -1.f;  // a little below the best quotient so far
-#pragma unroll 1
+#pragma unroll 2
     for (int i = tid; i < nvec; i += kThreads) {
       const uint4 w = *reinterpret_cast<const uint4*>(stage + i * VE);
       if (Vec<T>::largest(w) < least) continue;
       const T* v = reinterpret_cast<const T*>(&w);
-      float en[VE];
-      const bool wide = vec && least == -INFINITY && (i + 1) * VE <= n;  // all tokens are kept
-      if (wide)
+      alignas(16) float en[VE];
+      if (vec && (i + 1) * VE <= n) {
 #pragma unroll
-        for (int q = 0; q < VE / 4; ++q)
-          *reinterpret_cast<uint4*>(en + 4 * q) = ld_stream_u4(e + i * VE + 4 * q);
+        for (int q = 0; q < VE / 4; ++q) *reinterpret_cast<uint4*>(en + 4 * q) = ld_stream_u4(e + i * VE + 4 * q);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) en[j] = i * VE + j < n ? __ldg(e + i * VE + j) : 1.f;
+      }
+      const float lead = __int_as_float(*reinterpret_cast<volatile int*>(&lead_s));
 #pragma unroll
       for (int j = 0; j < VE; ++j) {
-        const float x = to_f<T>(v[j]) + 0.f;
-        const int at = i * VE + j;
-        if (x < least || x == -INFINITY || before(cut, Token{x, lo + at})) continue;
-        const float wt_ = weight(x), ej = wide ? en[j] : __ldg(e + at);
-        if (wt_ < mp || (wt_ <= lead * ej && ej > 0.f)) continue;  // (behind)
-        const unsigned long long cand = ticket(wt_, ej, lo + at);
-        if (cand > best) best = cand, lead = __uint_as_float((uint32_t)(cand >> 32)) * 0.999999f;
+        const float x = to_f<T>(v[j]) + 0.f, q = __fdividef(weight(x), en[j]);
+        if (x >= least && (q > lead || en[j] > 0x1p125f)) {  // (there the quick quotient is 0)
+          const int at = i * VE + j;
+          if (!kept(x, at)) continue;
+          const unsigned long long cand = ticket(weight(x), en[j], lo + at);
+          if (cand >> 32 == 0) continue;
+          atomicMax(&best_s, cand);
+          atomicMax(&lead_s, __float_as_int(fminf(__uint_as_float((uint32_t)(cand >> 32)) * 0.999999f, 3e38f)));
+        }
       }
     }
+    __syncthreads();
+    best = best_s;
   }
   best = block_reduce(best, max64, scratch);
   if (tid == 0) red.best = best;
   cluster.sync();
-  if (rank == 0 && tid == 0) {
+#pragma unroll 1
+  for (int r = 0; r < C; ++r) best = max64(best, cluster.map_shared_rank(&red, r)->best);
+  if (best == 0) {  // every kept token's quotient is 0 (its noise infinite, negative or NaN): the first of them
+    each(least, [&](float v, int i) {
+      if (kept(v, i)) best = max64(best, 0xffffffffu - (unsigned)(lo + i));
+    });
+    best = block_reduce(best, max64, scratch);
+    cluster.sync();
+    if (tid == 0) red.best = best;
+    cluster.sync();
+#pragma unroll 1
     for (int r = 0; r < C; ++r) best = max64(best, cluster.map_shared_rank(&red, r)->best);
-    finish(best);
   }
+  if (rank == 0 && tid == 0) finish(best);
   cluster.sync();  // the others' shared memory stays until rank 0 has read it
 }
 
@@ -632,7 +693,7 @@ cudaError_t launch_t(const SampleArgs& a, cudaStream_t st) {
   while (C < kMaxCluster && ((int64_t)a.vocab * (int64_t)sizeof(T) > C * 65536ll || (int64_t)a.rows * C * 2 <= num_sms()))
     C *= 2;
   const int slice = (div_up(a.vocab, C) + 7) / 8 * 8;
-  const size_t smem = kSplit * kThreads * 4 + (size_t)slice * sizeof(T) + 16;
+  const size_t smem = kSplit * kThreads * 4 + 3 * kBins * 4 + (size_t)slice * sizeof(T) + 16;
   auto kern = sample_kernel<T>;
   if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
   cudaLaunchConfig_t cfg{};
