@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "status.h"
 
 namespace b200ep {
@@ -167,6 +169,18 @@ inline int num_sms() {
     sms = n > 0 ? n : 148;
   }
   return sms;
+}
+
+// Lets `kern` use up to `most` bytes (the same in every call) of dynamic shared memory on the current device.
+// `set`: the kernel's own array (static), so that only the first launch on a device makes the call.
+constexpr int kMaxSmemDevices = 16;
+inline cudaError_t allow_smem(const void* kern, std::atomic<bool> (&set)[kMaxSmemDevices], int most) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  if (dev < kMaxSmemDevices && set[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) return e;
+  if (dev < kMaxSmemDevices) set[dev].store(true, std::memory_order_relaxed);
+  return cudaSuccess;
 }
 
 template <typename... KArgs, typename... Args>

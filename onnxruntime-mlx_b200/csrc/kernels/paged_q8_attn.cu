@@ -851,7 +851,9 @@ cudaError_t launch_t(const PagedQ8& a, bool appended, cudaStream_t st) {
   using C = Cfg<T, D, CT, NT>;
   auto kern = paged_q8_attn_kernel<T, D, CT, NT>;
   const int smem = C::kRaw + (std::min(a.G, C::kHeads) * D + (a.rot ? 2 * a.half : 0)) * (int)sizeof(T);
-  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
+  static std::atomic<bool> allowed[kMaxSmemDevices];
+  const int most = C::kRaw + (C::kHeads * D + D) * (int)sizeof(T);
+  if (cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed, most)) return e;
   // one wave: the CTAs that the SM's 228 KB hold (1 KB of each is the system's)
   const int per_sm = std::min<int>(C::kCtasPerSm, 228 * 1024 / (smem + C::kStatic + 1024));
   const int grid = std::min(a.ctas, num_sms() * per_sm);

@@ -286,13 +286,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   };
   auto gather = [&]() {  // the CTAs' lists, where they fit, into the first CTA's; the number of their tokens
     cluster.sync();
-    int got = 0;
-    for (int r = 0; r < C; ++r) {
-      const Red* o = cluster.map_shared_rank(&red, r);
-      const int c = o->got;
-      if (rank == 0 && got + c <= kCap)
-        for (int i = tid; i < c; i += kThreads) all[got + i] = o->list[i];
-      got += c;
+    int c[kMaxCluster], got = 0;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) c[r] = r < C ? cluster.map_shared_rank(&red, r)->got : 0;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      if (rank == 0 && tid < c[r] && got + c[r] <= kCap) all[got + tid] = cluster.map_shared_rank(&red, r)->list[tid];
+      got += c[r];
     }
     __syncthreads();
     return got;
@@ -467,13 +467,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     // ---- 16 bins of d = m - v, the last one without an end
     const float w = by_mass ? fminf(fmaxf(1.0397208f * t, 1e-3f), 64.f) : 1.f, rw = 1.f / w;
     constexpr float kMagic = 8388608.f;  // + 2^23 rounds to a whole number, in the low bits
-    auto bin_of = [&](float v) { return __float_as_uint(fminf((m - v) * rw, (float)(kSplit - 1)) + kMagic) & 31u; };
+    auto spot = [&](float v) { return fmaf(m - v, rw, kMagic); };  // 2^23 + the bin
 #pragma unroll
     for (int b = 0; b < kSplit; ++b) col[b * kThreads + tid] = 0.f;
-    if (by_mass)
-      each(-INFINITY, [&](float v, int) { col[bin_of(v) * kThreads + tid] += weight(v); });
-    else
-      each(-INFINITY, [&](float v, int) { col[bin_of(v) * kThreads + tid] += v > -INFINITY ? 1.f : 0.f; });
+    {
+      uint8_t* mine_col = reinterpret_cast<uint8_t*>(col + tid);
+      auto slot = [&](float v) {  // (2^23's own bits leave the word)
+        return reinterpret_cast<float*>(mine_col + (__float_as_uint(fminf(spot(v), kMagic + (float)(kSplit - 1))) * (uint32_t)(kThreads * 4)));
+      };
+      static_assert(kThreads * 4 >= 512, "the shift of the exponent bits");
+      if (by_mass)
+        each(-INFINITY, [&](float v, int) { *slot(v) += weight(v); });
+      else
+        each(-INFINITY, [&](float v, int) { *slot(v) += v > -INFINITY ? 1.f : 0.f; });
+    }
     __syncthreads();
     float s = 0.f;
 #pragma unroll
@@ -508,9 +515,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     const float rest = want - above;
     const unsigned long long need = by_mass ? (unsigned long long)((double)want * 4294967296.0) : 0;
     const float least = at == kSplit - 1 ? -INFINITY : m - ((float)at + 0.501f) * w;  // no token of the bins is smaller
+    // what spot() gives for the tokens of bin `at` (-infinity gives infinity)
+    const float spot0 = kMagic + (float)at, spot1 = at == kSplit - 1 ? 3e38f : spot0;
     int got = kCap + 1;
     if (whole) {
-      got = collect(least, [&](float v) { return v > -INFINITY && (int)bin_of(v) <= at; });
+      got = collect(least, [&](float v) { return spot(v) <= spot1; });
       if (got > kCap) cluster.sync();  // (before the lists are used again)
     }
     if (got > kCap) {
@@ -530,15 +539,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
         const int i = i0 + lane;
         const uint4 w4 = i < nvec ? *reinterpret_cast<const uint4*>(stage + i * VE) : uint4{};
         const T* v = reinterpret_cast<const T*>(&w4);
+        uint32_t in = 0;  // which of the thread's VE tokens
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-          const float x = to_f<T>(v[j]);
-          const bool in = i < nvec && x > -INFINITY && (int)bin_of(x) == at;
-          const uint32_t mask = __ballot_sync(0xffffffffu, in);
-          const int to = mine_n + __popc(mask & ((1u << lane) - 1u));
-          if (in && to < kNear) near[to] = (uint16_t)(i * VE + j);
-          mine_n += __popc(mask);
+          const float sp = spot(to_f<T>(v[j]));
+          if (sp >= spot0 && sp <= spot1) in |= 1u << j;
         }
+        if (i >= nvec) in = 0;
+        const int own = __popc(in);
+        int to = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, to, o);
+          if (lane >= o) to += u;
+        }
+        const int all_n = __shfl_sync(0xffffffffu, to, 31);
+        to += mine_n - own;
+        for (; in && to < kNear; in &= in - 1) near[to++] = (uint16_t)(i * VE + __ffs((int)in) - 1);
+        mine_n += all_n;
       }
       clear();
       auto visit = [&](auto f) {
@@ -547,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
           for (int q = lane; q < mine_n; q += 32) f(to_f<T>(stage[near[q]]) + 0.f, (int)near[q]);
         } else {  // too many: from the slice (a warp's vectors are the ones it listed)
           each(least, [&](float v, int i) {
-            if (v > -INFINITY && (int)bin_of(v) == at) f(v, i);
+            if (spot(v) >= spot0 && spot(v) <= spot1) f(v, i);
           });
         }
       };
@@ -632,11 +650,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   } else {
     // All threads share the best quotient so far, a little lowered (lead_s): few tokens come near it, so the
     // division that decides, and the tests of what is kept, run for those only.
-    if (tid == 0) best_s = 0, lead_s = 0;
-    __syncthreads();
     const float* e = noise + lo;
     const bool vec = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
-#pragma unroll 2
+    float first = 0.f;  // from each thread's first tokens
+    if (tid < nvec) {
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        const int at = tid * VE + j;
+        const float x = to_f<T>(stage[at]) + 0.f;
+        if (at < n && x >= least && kept(x, at)) {
+          const float q = __fdividef(weight(x), __ldg(e + at));
+          if (q < 3e38f) first = fmaxf(first, q);
+        }
+      }
+    }
+    first = block_reduce(first, [](float p, float q) { return fmaxf(p, q); }, reinterpret_cast<float*>(scratch));
+    if (tid == 0) best_s = 0, lead_s = __float_as_int(first * 0.9999f);
+    __syncthreads();
+#pragma unroll 1
     for (int i = tid; i < nvec; i += kThreads) {
       const uint4 w = *reinterpret_cast<const uint4*>(stage + i * VE);
       if (Vec<T>::largest(w) < least) continue;
@@ -650,17 +681,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
         for (int j = 0; j < VE; ++j) en[j] = i * VE + j < n ? __ldg(e + i * VE + j) : 1.f;
       }
       const float lead = __int_as_float(*reinterpret_cast<volatile int*>(&lead_s));
+      bool near_lead = false;  // (w / e > lead; a negative or NaN e is no matter here)
 #pragma unroll
+      for (int j = 0; j < VE; ++j) near_lead |= weight(to_f<T>(v[j])) > lead * en[j];
+      if (!near_lead) continue;
+#pragma unroll 1
       for (int j = 0; j < VE; ++j) {
-        const float x = to_f<T>(v[j]) + 0.f, q = __fdividef(weight(x), en[j]);
-        if (x >= least && (q > lead || en[j] > 0x1p125f)) {  // (there the quick quotient is 0)
-          const int at = i * VE + j;
-          if (!kept(x, at)) continue;
-          const unsigned long long cand = ticket(weight(x), en[j], lo + at);
-          if (cand >> 32 == 0) continue;
-          atomicMax(&best_s, cand);
-          atomicMax(&lead_s, __float_as_int(fminf(__uint_as_float((uint32_t)(cand >> 32)) * 0.999999f, 3e38f)));
-        }
+        const float x = to_f<T>(stage[i * VE + j]) + 0.f;
+        const int at = i * VE + j;
+        if (at >= n || !kept(x, at)) continue;
+        const unsigned long long cand = ticket(weight(x), __ldg(e + at), lo + at);
+        if (cand >> 32 == 0 || cand <= best) continue;
+        best = cand;
+        atomicMax(&best_s, cand);
+        atomicMax(&lead_s, __float_as_int(fminf(__uint_as_float((uint32_t)(cand >> 32)) * 0.9999f, 3e38f)));
       }
     }
     __syncthreads();
@@ -693,9 +727,12 @@ cudaError_t launch_t(const SampleArgs& a, cudaStream_t st) {
   while (C < kMaxCluster && ((int64_t)a.vocab * (int64_t)sizeof(T) > C * 65536ll || (int64_t)a.rows * C * 2 <= num_sms()))
     C *= 2;
   const int slice = (div_up(a.vocab, C) + 7) / 8 * 8;
-  const size_t smem = kSplit * kThreads * 4 + 3 * kBins * 4 + (size_t)slice * sizeof(T) + 16;
+  constexpr int kFixed = kSplit * kThreads * 4 + 3 * kBins * 4 + 16;
+  const size_t smem = kFixed + (size_t)slice * sizeof(T);
   auto kern = sample_kernel<T>;
-  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
+  static std::atomic<bool> allowed[kMaxSmemDevices];
+  constexpr int kMost = kFixed + (int)(kMaxVocab / kMaxCluster * sizeof(T));
+  if (cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed, kMost)) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.rows * C));
   cfg.blockDim = dim3(kThreads);

@@ -49,10 +49,18 @@ class PagedQ8Params(ctypes.Structure):
 _configured = False
 
 
+_TYPE = {}   # torch dtype -> ONNX TensorProto code, of rows
+_CACHE = {}  # ... and of 8-bit caches
+
+
 def _lib():
-    global _configured
+    global _configured, torch
     L = load_library()
     if not _configured:
+        import torch
+
+        _TYPE.update({torch.float32: 1, torch.float16: 10, torch.bfloat16: 16})
+        _CACHE.update({torch.int8: 3, torch.float8_e4m3fn: 17})
         vp, i64, i32, f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
         L.b200ep_matmulnbits.argtypes = [vp, vp, vp, vp, vp, i32, i64, i64, i64, i32, i32, vp]
         L.b200ep_matmulnbits_dequant.argtypes = [vp, vp, vp, vp, i32, i32, i64, i64, i32, i32, vp]
@@ -263,61 +271,91 @@ def paged_attention(query, key, value, key_cache, value_cache, cumulative_seqlen
     return out
 
 
-def _q8_params(key_cache, value_cache, key_scales, value_scales, block_table, batch, cos_cache=None, interleaved=0):
-    """The cache's geometry, checked the way the kernels rely on it."""
-    import torch
+# The bindings of the 8-bit cache and of sampling run once per decode step and layer: they check with few
+# attribute reads, hand addresses to ctypes as integers, and keep the parameter structs of geometries seen.
+_q8_structs = {}
 
-    types = {torch.int8: 3, torch.float8_e4m3fn: 17}
-    if key_cache.dtype not in types or value_cache.dtype != key_cache.dtype:
-        raise ValueError("paged 8-bit cache: key_cache and value_cache must both be int8 or float8_e4m3fn")
-    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
-        raise ValueError("paged 8-bit cache: caches must be [num_blocks, kv_heads, block_size, head_size]")
-    for s in (key_scales, value_scales):
-        if s.dtype != torch.float32 or s.shape != key_cache.shape[:3]:
-            raise ValueError("paged 8-bit cache: scales must be float32 [num_blocks, kv_heads, block_size]")
+
+def _q8_fail(what):
+    raise ValueError("paged 8-bit cache: " + what)
+
+
+def _q8_cache(key_cache, value_cache, key_scales, value_scales, block_table, batch):
+    """Checks the cache's tensors the way the kernels rely on them; returns the pages' shape."""
+    shape, dtype = key_cache.shape, key_cache.dtype
+    if dtype not in _CACHE or value_cache.dtype != dtype:
+        _q8_fail("key_cache and value_cache must both be int8 or float8_e4m3fn")
+    if len(shape) != 4 or value_cache.shape != shape:
+        _q8_fail("caches must be [num_blocks, kv_heads, block_size, head_size]")
+    rows = shape[:3]
+    if key_scales.shape != rows or value_scales.shape != rows or key_scales.dtype != torch.float32 or (
+            value_scales.dtype != torch.float32):
+        _q8_fail("scales must be float32 [num_blocks, kv_heads, block_size]")
     if not (key_cache.is_contiguous() and value_cache.is_contiguous() and key_scales.is_contiguous()
             and value_scales.is_contiguous()):
-        raise ValueError("paged 8-bit cache: caches and scales must be contiguous")
+        _q8_fail("caches and scales must be contiguous")
     if block_table.dtype != torch.int32 or not block_table.is_contiguous() or (
             batch and block_table.numel() % batch):
-        raise ValueError("paged 8-bit cache: block_table must be a contiguous int32 [batch, max_blocks]")
-    p = PagedQ8Params()
-    p.num_blocks, p.kv_heads, p.block_size, p.head_size = key_cache.shape
-    p.batch = batch
-    p.max_blocks = block_table.numel() // batch if batch else 1
-    p.cache_type = types[key_cache.dtype]
-    if cos_cache is not None:
-        p.do_rotary, p.interleaved = 1, int(interleaved)
-        p.max_seq, p.rotary_half = cos_cache.shape
-    return p
+        _q8_fail("block_table must be a contiguous int32 [batch, max_blocks]")
+    return shape
 
 
-def _q8_rows(name, x, width, dtype=None, tokens=None):
+def _q8_rows(name, x, width, dtype, tokens):
     """Packed rows [T, width]; the rows may be slices of wider ones.  Returns the row stride."""
-    if x.dim() != 2 or x.shape[1] != width or (tokens is not None and x.shape[0] != tokens):
-        raise ValueError(f"paged 8-bit cache: {name} must be [{'T' if tokens is None else tokens}, {width}]")
-    if dtype is not None and x.dtype != dtype:
-        raise ValueError(f"paged 8-bit cache: {name} must be {dtype}")
-    if x.shape[0] > 1 and (x.stride(1) != 1 or x.stride(0) < width) or x.shape[0] == 1 and x.stride(1) != 1:
-        raise ValueError(f"paged 8-bit cache: the elements of a row of {name} must be contiguous")
-    return x.stride(0) if x.shape[0] > 1 else width
+    if x.shape != (tokens, width):
+        _q8_fail(f"{name} must be [{tokens}, {width}]")
+    if x.dtype != dtype:
+        _q8_fail(f"{name} must be {dtype}")
+    row, one = x.stride()
+    if one != 1 or tokens > 1 and row < width:
+        _q8_fail(f"the elements of a row of {name} must be contiguous")
+    return row if tokens > 1 else width
 
 
 def _q8_control(cumulative_seqlens, past_seqlens, cos_cache, sin_cache, dtype):
-    import torch
+    """Checks lengths and angles; returns (sequences, rows and columns of the cos / sin caches)."""
+    batch = past_seqlens.numel()
+    if cumulative_seqlens.dtype != torch.int32 or not cumulative_seqlens.is_contiguous():
+        _q8_fail("cumulative_seqlens must be contiguous int32")
+    if past_seqlens.dtype != torch.int32 or not past_seqlens.is_contiguous():
+        _q8_fail("past_seqlens must be contiguous int32")
+    if cumulative_seqlens.numel() != batch + 1:
+        _q8_fail("cumulative_seqlens must have one entry more than past_seqlens")
+    if cos_cache is None or sin_cache is None:
+        if cos_cache is not sin_cache:
+            _q8_fail("cos_cache and sin_cache come together")
+        return batch, 0, 0
+    shape = cos_cache.shape
+    if cos_cache.dtype != dtype or sin_cache.dtype != dtype or len(shape) != 2 or sin_cache.shape != shape or not (
+            cos_cache.is_contiguous() and sin_cache.is_contiguous()):
+        _q8_fail("cos / sin must be contiguous [max_seq, rotary_half] of the rows' type")
+    return batch, shape[0], shape[1]
 
-    for name, t in (("cumulative_seqlens", cumulative_seqlens), ("past_seqlens", past_seqlens)):
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise ValueError(f"paged 8-bit cache: {name} must be contiguous int32")
-    if cumulative_seqlens.numel() != past_seqlens.numel() + 1:
-        raise ValueError("paged 8-bit cache: cumulative_seqlens must have one entry more than past_seqlens")
-    if (cos_cache is None) != (sin_cache is None):
-        raise ValueError("paged 8-bit cache: cos_cache and sin_cache come together")
-    if cos_cache is not None:
-        for t in (cos_cache, sin_cache):
-            if t.dtype != dtype or t.shape != cos_cache.shape or t.dim() != 2 or not t.is_contiguous():
-                raise ValueError("paged 8-bit cache: cos / sin must be contiguous [max_seq, rotary_half] of the "
-                                 "rows' type")
+
+def _q8_struct(batch, tokens, heads, pages, cache_type, max_blocks, max_seq, half, interleaved, scale, strides):
+    key = (batch, tokens, heads, pages, cache_type, max_blocks, max_seq, half, interleaved, scale, strides)
+    ref = _q8_structs.get(key)
+    if ref is None:
+        if len(_q8_structs) >= 4096:  # (every batch size and prompt length is a geometry)
+            _q8_structs.clear()
+        blocks, kv_heads, block, head = pages
+        ref = _q8_structs[key] = ctypes.byref(PagedQ8Params(
+            batch, tokens, heads, kv_heads, head, blocks, block, max_blocks, max_seq, half, int(half > 0),
+            int(interleaved), cache_type, scale, *strides))
+    return ref
+
+
+def _device(*tensors):
+    """The CUDA device that all of the tensors are on."""
+    at = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != at or at < 0:
+            raise ValueError("the tensors must be on one CUDA device")
+    return at
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def paged_kv_quantize(key, value, key_cache, value_cache, key_scales, value_scales, cumulative_seqlens,
@@ -325,17 +363,20 @@ def paged_kv_quantize(key, value, key_cache, value_cache, key_scales, value_scal
     """Write packed key / value rows [T, kv_heads * D] (the key after RoPE) into 8-bit pages, in place:
     codes [num_blocks, kv_heads, block_size, D] int8 or float8_e4m3fn, scales float32
     [num_blocks, kv_heads, block_size].  Rows may be slices of a packed projection."""
-    p = _q8_params(key_cache, value_cache, key_scales, value_scales, block_table, past_seqlens.numel(), cos_cache,
-                   interleaved)
-    _q8_control(cumulative_seqlens, past_seqlens, cos_cache, sin_cache, key.dtype)
-    width = p.kv_heads * p.head_size
-    p.key_stride = _q8_rows("key", key, width)
-    p.value_stride = _q8_rows("value", value, width, key.dtype, key.shape[0])
-    p.num_tokens = key.shape[0]
-    check(_lib().b200ep_paged_kv_quantize(
-        ctypes.byref(p), _p(key), _p(value), _p(key_cache), _p(value_cache), _p(key_scales), _p(value_scales),
-        _p(cumulative_seqlens), _p(past_seqlens), _p(block_table), _p(cos_cache), _p(sin_cache), _dt(key),
-        _stream(key.device)))
+    L = _lib()
+    dtype = key.dtype
+    batch, max_seq, half = _q8_control(cumulative_seqlens, past_seqlens, cos_cache, sin_cache, dtype)
+    pages = _q8_cache(key_cache, value_cache, key_scales, value_scales, block_table, batch)
+    T, width = key.shape[0], pages[1] * pages[3]
+    strides = (0, _q8_rows("key", key, width, dtype, T), _q8_rows("value", value, width, dtype, T))
+    p = _q8_struct(batch, T, 0, pages, _CACHE[key_cache.dtype], block_table.numel() // batch if batch else 1, max_seq,
+                   half, interleaved, 0.0, strides)
+    device = _device(key, value, key_cache, value_cache, key_scales, value_scales, cumulative_seqlens, past_seqlens,
+                     block_table)
+    check(L.b200ep_paged_kv_quantize(
+        p, key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+        value_scales.data_ptr(), cumulative_seqlens.data_ptr(), past_seqlens.data_ptr(), block_table.data_ptr(),
+        half and cos_cache.data_ptr(), half and sin_cache.data_ptr(), _TYPE.get(dtype, 0), _raw_stream(device)))
 
 
 def paged_kv_dequantize(key_cache, value_cache, key_scales, value_scales, seqlens, block_table, *, cap=None,
@@ -343,28 +384,32 @@ def paged_kv_dequantize(key_cache, value_cache, key_scales, value_scales, seqlen
     """Read the first seqlens[b] positions of each sequence out of 8-bit pages: (key, value), each
     [B, kv_heads, cap, D] of ``dtype`` with zeros from seqlens[b] on — GroupQueryAttention's shared-buffer
     layout.  ``cap`` and ``dtype`` are taken from ``key`` / ``value`` when those are given."""
-    import torch
-
-    B = seqlens.numel()
-    p = _q8_params(key_cache, value_cache, key_scales, value_scales, block_table, B)
+    L = _lib()
     if seqlens.dtype != torch.int32 or not seqlens.is_contiguous():
-        raise ValueError("paged 8-bit cache: seqlens must be contiguous int32")
-    if (key is None) != (value is None):
-        raise ValueError("paged 8-bit cache: key and value come together")
-    if key is None:
+        _q8_fail("seqlens must be contiguous int32")
+    B = seqlens.numel()
+    pages = _q8_cache(key_cache, value_cache, key_scales, value_scales, block_table, B)
+    if key is None and value is None:
         if cap is None:
-            raise ValueError("paged 8-bit cache: cap is needed when no output is given")
-        shape = (B, p.kv_heads, cap, p.head_size)
+            _q8_fail("cap is needed when no output is given")
+        shape = (B, pages[1], cap, pages[3])
+        device = _device(key_cache, value_cache, key_scales, value_scales, seqlens, block_table)
         key = torch.empty(shape, dtype=dtype or torch.float16, device=key_cache.device)
         value = torch.empty_like(key)
     else:
+        if key is None or value is None:
+            _q8_fail("key and value come together")
         cap = key.shape[2] if key.dim() == 4 else -1
-        if key.shape != (B, p.kv_heads, cap, p.head_size) or value.shape != key.shape or (
+        if key.shape != (B, pages[1], cap, pages[3]) or value.shape != key.shape or (
                 value.dtype != key.dtype) or not (key.is_contiguous() and value.is_contiguous()):
-            raise ValueError("paged 8-bit cache: outputs must be contiguous [B, kv_heads, cap, D] of one type")
-    check(_lib().b200ep_paged_kv_dequantize(
-        ctypes.byref(p), _p(key_cache), _p(value_cache), _p(key_scales), _p(value_scales), _p(seqlens),
-        _p(block_table), _p(key), _p(value), cap, _dt(key), _stream(key.device)))
+            _q8_fail("outputs must be contiguous [B, kv_heads, cap, D] of one type")
+        device = _device(key_cache, value_cache, key_scales, value_scales, seqlens, block_table, key, value)
+    p = _q8_struct(B, 0, 0, pages, _CACHE[key_cache.dtype], block_table.numel() // B if B else 1, 0, 0, 0, 0.0,
+                   (0, 0, 0))
+    check(L.b200ep_paged_kv_dequantize(
+        p, key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+        seqlens.data_ptr(), block_table.data_ptr(), key.data_ptr(), value.data_ptr(), cap, _TYPE.get(key.dtype, 0),
+        _raw_stream(device)))
     return key, value
 
 
@@ -382,34 +427,49 @@ def paged_attention_quantized(query, key, value, key_cache, value_cache, key_sca
     are first written into the pages.  ``workspace``: a uint8 tensor of at least
     paged_attention_quantized_workspace_size bytes, any contents; allocated on the current stream when
     absent."""
-    import torch
-
-    p = _q8_params(key_cache, value_cache, key_scales, value_scales, block_table, past_seqlens.numel(), cos_cache,
-                   interleaved)
-    _q8_control(cumulative_seqlens, past_seqlens, cos_cache, sin_cache, query.dtype)
-    if p.kv_heads != kv_heads:
-        raise ValueError(f"paged 8-bit cache: the cache holds {p.kv_heads} kv heads, not {kv_heads}")
-    T, D = query.shape[0], p.head_size
-    p.num_heads, p.num_tokens, p.scale = num_heads, T, float(scale)
-    p.query_stride = _q8_rows("query", query, num_heads * D)
-    if (key is None) != (value is None):
-        raise ValueError("paged 8-bit cache: key and value come together, or neither")
-    if key is not None:
-        p.key_stride = _q8_rows("key", key, kv_heads * D, query.dtype, T)
-        p.value_stride = _q8_rows("value", value, kv_heads * D, query.dtype, T)
-    if out is None:
-        out = torch.empty(T, num_heads * D, dtype=query.dtype, device=query.device)
-    elif out.shape != (T, num_heads * D) or out.dtype != query.dtype or not out.is_contiguous():
-        raise ValueError("paged 8-bit cache: out must be contiguous [T, num_heads * D] of the query's type")
     L = _lib()
+    dtype = query.dtype
+    batch, max_seq, half = _q8_control(cumulative_seqlens, past_seqlens, cos_cache, sin_cache, dtype)
+    pages = _q8_cache(key_cache, value_cache, key_scales, value_scales, block_table, batch)
+    if pages[1] != kv_heads:
+        _q8_fail(f"the cache holds {pages[1]} kv heads, not {kv_heads}")
+    T, D = query.shape[0], pages[3]
+    strides = _q8_rows("query", query, num_heads * D, dtype, T)
+    if key is None and value is None:
+        strides = (strides, 0, 0)
+        device = _device(query, key_cache, value_cache, key_scales, value_scales, cumulative_seqlens, past_seqlens,
+                         block_table)
+    else:
+        if key is None or value is None:
+            _q8_fail("key and value come together, or neither")
+        strides = (strides, _q8_rows("key", key, kv_heads * D, dtype, T),
+                   _q8_rows("value", value, kv_heads * D, dtype, T))
+        device = _device(query, key_cache, value_cache, key_scales, value_scales, cumulative_seqlens, past_seqlens,
+                         block_table, key, value)
+    if out is None:
+        out = torch.empty((T, num_heads * D), dtype=dtype, device=query.device)
+    elif out.shape != (T, num_heads * D) or out.dtype != dtype or not out.is_contiguous():
+        _q8_fail("out must be contiguous [T, num_heads * D] of the query's type")
+    p = _q8_struct(batch, T, num_heads, pages, _CACHE[key_cache.dtype], block_table.numel() // batch if batch else 1,
+                   max_seq, half, interleaved, scale, strides)
     if workspace is None:
-        workspace = torch.empty(L.b200ep_paged_attention_quantized_workspace_size(ctypes.byref(p)),
-                                dtype=torch.uint8, device=query.device)
+        workspace = torch.empty(L.b200ep_paged_attention_quantized_workspace_size(p), dtype=torch.uint8,
+                                device=query.device)
     check(L.b200ep_paged_attention_quantized(
-        ctypes.byref(p), _p(query), _p(key), _p(value), _p(key_cache), _p(value_cache), _p(key_scales),
-        _p(value_scales), _p(cumulative_seqlens), _p(past_seqlens), _p(block_table), _p(cos_cache), _p(sin_cache),
-        _p(out), _dt(query), _p(workspace), workspace.numel() * workspace.element_size(), _stream(query.device)))
+        p, query.data_ptr(), key if key is None else key.data_ptr(), value if value is None else value.data_ptr(),
+        key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+        cumulative_seqlens.data_ptr(), past_seqlens.data_ptr(), block_table.data_ptr(),
+        half and cos_cache.data_ptr(), half and sin_cache.data_ptr(), out.data_ptr(), _TYPE.get(dtype, 0),
+        workspace.data_ptr(), workspace.nbytes, _raw_stream(device)))
     return out
+
+
+def _per_row(name, x, dtype, B):
+    if x is None:
+        return None
+    if x.dtype != dtype or x.shape != (B,) or not x.is_contiguous():
+        raise ValueError(f"sample: {name} must be contiguous {dtype} [{B}]")
+    return x.data_ptr()
 
 
 def sample(logits, noise, temperature=None, top_k=None, top_p=None, min_p=None, *, tokens=None, logprobs=None):
@@ -417,29 +477,28 @@ def sample(logits, noise, temperature=None, top_k=None, top_p=None, min_p=None, 
     [B, V] of standard exponential numbers (``torch.empty(B, V).exponential_()``).  ``temperature`` (0: the largest
     logit), ``top_k`` int32 (<= 0: all), ``top_p`` (>= 1: all) and ``min_p`` (<= 0: all) are [B] or None.  Rows may
     be slices of wider ones.  tokens is -1 where every logit is -inf or NaN."""
-    import torch
-
-    if logits.dim() != 2 or noise.shape != logits.shape:
+    L = _lib()
+    shape = logits.shape
+    if len(shape) != 2 or noise.shape != shape:
         raise ValueError("sample: logits and noise must both be [B, V]")
     if noise.dtype != torch.float32:
         raise ValueError("sample: noise must be float32")
-    B, V = logits.shape
-    for name, x in (("logits", logits), ("noise", noise)):
-        if V > 1 and x.stride(1) != 1 or B > 1 and x.stride(0) < V:
-            raise ValueError(f"sample: the elements of a row of {name} must be contiguous")
-    for name, x, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if x is not None and (x.dtype != dtype or x.shape != (B,) or not x.is_contiguous()):
-            raise ValueError(f"sample: {name} must be contiguous {dtype} [{B}]")
+    B, V = shape
+    (lr, lc), (nr, nc) = logits.stride(), noise.stride()
+    if V > 1 and (lc != 1 or nc != 1) or B > 1 and (lr < V or nr < V):
+        raise ValueError("sample: the elements of a row of logits and of noise must be contiguous")
+    f32 = torch.float32
+    args = (_per_row("temperature", temperature, f32, B), _per_row("top_k", top_k, torch.int32, B),
+            _per_row("top_p", top_p, f32, B), _per_row("min_p", min_p, f32, B))
+    if tokens is not None and (tokens.dtype != torch.int64 or tokens.numel() != B or not tokens.is_contiguous()):
+        raise ValueError(f"sample: tokens must be contiguous int64 with {B} entries")
+    if logprobs is not None and (logprobs.dtype != f32 or logprobs.shape != (B,) or not logprobs.is_contiguous()):
+        raise ValueError(f"sample: logprobs must be contiguous float32 [{B}]")
+    device = _device(logits, noise)
     if tokens is None:
         tokens = torch.empty(B, dtype=torch.int64, device=logits.device)
-    elif tokens.dtype != torch.int64 or tokens.numel() != B or not tokens.is_contiguous():
-        raise ValueError(f"sample: tokens must be contiguous int64 with {B} entries")
     if logprobs is None:
-        logprobs = torch.empty(B, dtype=torch.float32, device=logits.device)
-    elif logprobs.dtype != torch.float32 or logprobs.shape != (B,) or not logprobs.is_contiguous():
-        raise ValueError(f"sample: logprobs must be contiguous float32 [{B}]")
-    check(_lib().b200ep_sample(_p(logits), _p(noise), _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(tokens),
-                               _p(logprobs), B, V, logits.stride(0) if B > 1 else 0, noise.stride(0) if B > 1 else 0,
-                               _dt(logits), _stream(logits.device)))
+        logprobs = torch.empty(B, dtype=f32, device=logits.device)
+    check(L.b200ep_sample(logits.data_ptr(), noise.data_ptr(), *args, tokens.data_ptr(), logprobs.data_ptr(), B, V,
+                          lr if B > 1 else 0, nr if B > 1 else 0, _TYPE.get(logits.dtype, 0), _raw_stream(device)))
     return tokens, logprobs

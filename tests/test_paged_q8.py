@@ -487,6 +487,7 @@ def _call(ops, a):
     (dict(past=torch.zeros(2, dtype=torch.int64)), "past_seqlens"),
     (dict(cos=torch.zeros(9, 32, dtype=torch.float16)), "come together"),
     (dict(cos=torch.zeros(9, 32), sin=torch.zeros(9, 32)), "cos / sin"),
+    (dict(), "one CUDA device"),
 ])
 def test_refusals_of_the_binding(ops, kw, match):
     with pytest.raises(ValueError, match=match):
