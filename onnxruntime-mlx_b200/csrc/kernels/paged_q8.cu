@@ -9,7 +9,7 @@
 //   arithmetic.  a = 0 gives code 0 and scale 0; a row that holds an infinity or a NaN gets scale NaN
 //   and reads back as NaN.
 //   D / 8 lanes hold one row, 8 elements each: one 16-byte load (16-bit types), an xor-shuffle maximum,
-//   one 8-byte store.  Keys and values of a token are handled by one CTA.
+//   one 8-byte store.
 // paged_q8_read_kernel — sequences gathered into [B, HK, cap, D] rows of a float type (the layout of
 //   GroupQueryAttention's shared buffers); rows at and past a sequence's length are zeros.
 // Both are bound by HBM: 2 B + 1 B (+ 4 / D) per element each way for 16-bit types.
@@ -21,10 +21,6 @@
 
 namespace b200ep {
 namespace {
-
-__device__ __forceinline__ void store_bytes8(uint8_t* dst, uint32_t a, uint32_t b) {
-  *reinterpret_cast<uint2*>(dst) = make_uint2(a, b);
-}
 
 // 8 consecutive elements to fp32; `vec`: the address is 16-byte aligned.
 template <typename T>
@@ -42,11 +38,10 @@ __device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
   }
 }
 
-// RoPE of the 8 elements [d0, d0 + 8) of a row held 8 per lane by D / 8 lanes; every lane of the row
-// takes part.  Products and sums are rounded one by one (no fused multiply-add), as PagedAttention
-// rounds them.
+// RoPE of the 8 elements [d0, d0 + 8) of a row, in pairs (2i, 2i + 1) or from halves of any length.  Products and
+// sums are rounded one by one (no fused multiply-add), as PagedAttention rounds them.
 template <typename T, int D>
-__device__ __forceinline__ void rope8(float (&x)[8], const T* row, int d0, const PagedQ8& kp, int pos, bool cvec) {
+__device__ __forceinline__ void rope8(float (&x)[8], const T* row, int d0, const PagedQ8& kp, int pos) {
   const T* C = static_cast<const T*>(kp.cos_c) + (size_t)pos * kp.half;
   const T* S = static_cast<const T*>(kp.sin_c) + (size_t)pos * kp.half;
   if (kp.inter) {  // pairs (2i, 2i + 1) lie in one lane
@@ -60,24 +55,6 @@ __device__ __forceinline__ void rope8(float (&x)[8], const T* row, int d0, const
     }
     return;
   }
-  if (kp.half % 8 == 0) {  // the partner's 8 elements are another lane's
-    const bool in = d0 < 2 * kp.half, first = d0 < kp.half;
-    const int step = kp.half / 8, lane = threadIdx.x & (D / 8 - 1);
-    const int src = !in ? lane : first ? lane + step : lane - step;
-    float y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], src, D / 8);
-    if (!in) return;
-    float c[8], s[8];
-    const int i0 = first ? d0 : d0 - kp.half;
-    load8<T>(C + i0, cvec, c);
-    load8<T>(S + i0, cvec, s);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      x[e] = first ? __fsub_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]))
-                   : __fadd_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]));
-    return;
-  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {  // any other half: the partner is read again
     const int i = d0 + e;
@@ -89,85 +66,165 @@ __device__ __forceinline__ void rope8(float (&x)[8], const T* row, int d0, const
   }
 }
 
+// x F / amax to codes, 8 of them.  The quick quotient x r, r = F / amax, is within 2^-22 of the true one: where that
+// cannot move any of them over a rounding point it decides, else the division does.  Adding 1.5 2^23 rounds to a whole
+// number whose low byte is the code (the conversion instructions run at an eighth of the rate).
 template <int CT>
-__device__ __forceinline__ uint32_t code_of(float x, float amax) {
+__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float amax, float r) {
+  uint32_t w[2];
+  bool near_tie = false;
   if constexpr (CT == kI8) {
-    return (uint32_t)__float2int_rn(__fdiv_rn(__fmul_rn(x, 127.f), amax)) & 0xffu;
+    constexpr float kMagic = 12582912.f;
+    float y[8], off = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float t = __fmul_rn(x[e], r);
+      y[e] = __fadd_rn(t, kMagic);
+      off = fmaxf(off, fabsf(__fsub_rn(t, __fsub_rn(y[e], kMagic))));
+    }
+    near_tie = !(off < 0.4999f);
+    if (near_tie)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = __fadd_rn(__fdiv_rn(__fmul_rn(x[e], 127.f), amax), kMagic);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const uint32_t* b = reinterpret_cast<const uint32_t*>(y + 4 * q);
+      w[q] = prmt(prmt(b[0], b[1], 0x0040), prmt(b[2], b[3], 0x0040), 0x5410);
+    }
   } else {
-    return __nv_cvt_float_to_fp8(__fdiv_rn(__fmul_rn(x, 448.f), amax), __NV_SATFINITE, __NV_E4M3);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float2 t = make_float2(__fmul_rn(x[e], r), __fmul_rn(x[e + 1], r));
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t.x * 0.9999995f, t.y * 0.9999995f), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t.x * 1.0000005f, t.y * 1.0000005f), __NV_SATFINITE, __NV_E4M3);
+      near_tie |= lo != hi;
+      w[e >> 2] = e & 2 ? prmt(w[e >> 2], lo, 0x5410) : lo;
+    }
+    if (near_tie)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const uint32_t c = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(__fmul_rn(x[e], 448.f), amax),
+                                                                __fdiv_rn(__fmul_rn(x[e + 1], 448.f), amax)),
+                                                    __NV_SATFINITE, __NV_E4M3);
+        w[e >> 2] = e & 2 ? prmt(w[e >> 2], c, 0x5410) : c;
+      }
   }
+  return make_uint2(w[0], w[1]);
 }
 
-constexpr int kWriteThreads = 128;
+constexpr int kWriteThreads = 256;
 
-template <typename T, int D, int CT>
+// The rows of all tokens as one list (the HK key rows of a token, then its HK value rows), kWriteThreads / (D / 8)
+// x U of them a CTA: the page rows of a CTA's tokens are looked up once, and each thread has all its
+// loads on their way before it uses the first.
+template <typename T, int D, int CT, int U>
 __global__ void __launch_bounds__(kWriteThreads) paged_q8_write_kernel(PagedQ8 kp, int vec) {
-  constexpr int L = D / 8;  // lanes of a row
+  constexpr int L = D / 8, PER = kWriteThreads / L, ROWS = PER * U;  // lanes of a row; rows
   constexpr float F = CT == kI8 ? 127.f : 448.f;
+  constexpr int VB = sizeof(T) / 2;  // 16-byte loads of 8 elements
+  __shared__ int2 tok_s[ROWS];       // a token's page row (-1: none) and position
   pdl_wait();
   pdl_trigger();
-  const int i = blockIdx.x;
-  if (kp.counters && i == 0)  // the attention launch that follows counts arrivals from zero
+  if (kp.counters && blockIdx.x == 0)  // the attention launch that follows counts arrivals from zero
     for (int t = threadIdx.x; t < kp.ctas; t += kWriteThreads) kp.counters[t] = 0;
-  const int b = q8_seq(kp.cum, kp.batch, i);
-  const int pos = b >= 0 ? __ldg(kp.past + b) + (i - __ldg(kp.cum + b)) : -1;
-  const bool pos_ok = pos >= 0 && !(kp.rot && pos >= kp.max_seq);
-  const int row0 = pos_ok ? q8_row(kp.bt, kp.maxb, kp.nblocks, kp.bs, kp.HK, b, 0, pos) : -1;
-  if (row0 < 0) {
-    if (threadIdx.x == 0) report_device_error(kp.err, kErrPagedQ8, i);
-    return;
-  }
+  const uint32_t r0 = blockIdx.x * ROWS, total = (uint32_t)kp.ntok * 2 * kp.HK, hk2 = 2 * kp.HK;  // (below 2^31)
+  const int first = (int)(r0 / hk2);
+  const int ntok = (int)((min(total, r0 + ROWS) - 1) / hk2) - first + 1;
   const int lane = threadIdx.x & (L - 1), d0 = lane * 8;
-  // row r < HK: the key row of kv head r; then the value rows.  All lanes of a warp stay in the loop
-  // (the shuffles name the full warp).
-  const int rows = 2 * kp.HK, per = kWriteThreads / L;
-  for (int r0 = 0; r0 < rows; r0 += per) {
-    const int r = r0 + (int)threadIdx.x / L;
-    const bool live = r < rows, is_k = r < kp.HK;
-    const int h = !live ? 0 : is_k ? r : r - kp.HK;
-    const T* src = (is_k || !live ? static_cast<const T*>(kp.k) + (size_t)i * kp.ks
-                                  : static_cast<const T*>(kp.v) + (size_t)i * kp.vs) + (size_t)h * D;
+  uint4 raw[U][VB];
+  int tok[U], head[U];  // token (from `first`; -1: past the end); key head, or HK + value head
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t r = r0 + u * PER + threadIdx.x / L;
+    const int i = r < total ? (int)(r / hk2) : 0;
+    tok[u] = r < total ? i - first : -1;
+    head[u] = r < total ? (int)(r - i * hk2) : 0;
+    const bool is_k = head[u] < kp.HK;
+    const T* src = (is_k ? static_cast<const T*>(kp.k) + (size_t)i * kp.ks + (size_t)head[u] * D
+                         : static_cast<const T*>(kp.v) + (size_t)i * kp.vs + (size_t)(head[u] - kp.HK) * D) + d0;
+    if (vec & 1) {
+#pragma unroll
+      for (int w = 0; w < VB; ++w) raw[u][w] = __ldg(reinterpret_cast<const uint4*>(src) + w);
+    } else {
+      T* e = reinterpret_cast<T*>(raw[u]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = src[j];
+    }
+  }
+  if ((int)threadIdx.x < ntok) {
+    const int i = first + threadIdx.x;
+    const int b = q8_seq(kp.cum, kp.batch, i);
+    const int pos = b >= 0 ? __ldg(kp.past + b) + (i - __ldg(kp.cum + b)) : -1;
+    const bool ok = pos >= 0 && !(kp.rot && pos >= kp.max_seq);
+    const int row = ok ? q8_row(kp.bt, kp.maxb, kp.nblocks, kp.bs, kp.HK, b, 0, pos) : -1;
+    if (row < 0) report_device_error(kp.err, kErrPagedQ8, i);
+    tok_s[threadIdx.x] = make_int2(row, pos);
+  }
+  __syncthreads();
+  // halves of whole 8-element chunks, aligned rows: the partner's elements are another lane's, and the angles of
+  // all rows are on their way before the first is used
+  const bool wide = kp.rot && (vec & 2);
+  const bool turned = d0 < 2 * kp.half, lower = d0 < kp.half;
+  uint4 cs[U][VB], sn[U][VB];
+  if (wide && turned)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int pos = tok[u] >= 0 && tok_s[tok[u]].x >= 0 ? tok_s[tok[u]].y : -1;
+      if (pos < 0 || head[u] >= kp.HK) continue;
+      const size_t o = (size_t)pos * kp.half + (lower ? d0 : d0 - kp.half);
+#pragma unroll
+      for (int w = 0; w < VB; ++w) {
+        cs[u][w] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(kp.cos_c) + o) + w);
+        sn[u][w] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(kp.sin_c) + o) + w);
+      }
+    }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {  // (all lanes of a warp take part in the shuffles)
+    const int2 at = tok[u] >= 0 ? tok_s[tok[u]] : make_int2(-1, 0);
+    const bool is_k = head[u] < kp.HK;
+    const int h = is_k ? head[u] : head[u] - kp.HK;
     float x[8];
-    load8<T>(src + d0, vec & 1, x);
-    if (kp.rot) {
-      float y[8];
+    {
+      const T* e = reinterpret_cast<const T*>(raw[u]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = x[e];
-      rope8<T, D>(y, src, d0, kp, pos, vec & 2);
-      if (is_k)
+      for (int j = 0; j < 8; ++j) x[j] = to_f<T>(e[j]);
+    }
+    if (wide) {
+      if (__any_sync(0xffffffffu, is_k && at.x >= 0)) {
+        const int step = kp.half / 8, from = !turned ? lane : lower ? lane + step : lane - step;
+        const T *c = reinterpret_cast<const T*>(cs[u]), *s = reinterpret_cast<const T*>(sn[u]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = y[e];
+        for (int e = 0; e < 8; ++e) {
+          // (both of a pair exchange before either is replaced: element e of all lanes at once)
+          const float y = __shfl_sync(0xffffffffu, x[e], from, L);
+          if (is_k && turned && at.x >= 0) {
+            const float a = __fmul_rn(x[e], to_f<T>(c[e])), b = __fmul_rn(y, to_f<T>(s[e]));
+            x[e] = lower ? __fsub_rn(a, b) : __fadd_rn(a, b);
+          }
+        }
+      }
+    } else if (kp.rot && is_k && at.x >= 0) {
+      rope8<T, D>(x, static_cast<const T*>(kp.k) + (size_t)(first + tok[u]) * kp.ks + (size_t)h * D, d0, kp, at.y);
     }
     uint32_t m = 0;  // |x| as bits: ordered like the values, a NaN above all
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (!live) continue;
+    if (at.x < 0) continue;
     float amax = __uint_as_float(m), scale = __fdiv_rn(amax, F);
     if (m >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u);
-    if (amax > 1e30f) {  // x F stays finite (a power of two: exact)
-      amax *= 0x1p-32f;
+    if (amax > 1e30f || amax < 1e-30f) {  // x F and F / amax stay in range (a power of two: exact)
+      const float s = amax > 1.f ? 0x1p-32f : 0x1p64f;
+      amax *= s;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= 0x1p-32f;
+      for (int e = 0; e < 8; ++e) x[e] *= s;
     }
-    uint32_t w[2] = {0, 0};
-    if (m)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e >> 2] |= code_of<CT>(x[e], amax) << (8 * (e & 3));
-    const int64_t row = row0 + (int64_t)h * kp.bs;
-    store_bytes8((is_k ? kp.kc : kp.vc) + row * D + d0, w[0], w[1]);
+    uint2 w = make_uint2(0, 0);
+    if (m && m < 0x7f800000u) w = codes_of<CT>(x, amax, __fdiv_rn(F, amax));
+    const int64_t row = at.x + (int64_t)h * kp.bs;
+    *reinterpret_cast<uint2*>((is_k ? kp.kc : kp.vc) + row * D + d0) = w;
     if (lane == 0) (is_k ? kp.kscale : kp.vscale)[row] = scale;
-  }
-}
-
-// one code to its value (before the scale)
-template <int CT>
-__device__ __forceinline__ float value_of(uint32_t byte) {
-  if constexpr (CT == kI8) {
-    return (float)(int8_t)byte;
-  } else {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
   }
 }
 
@@ -176,36 +233,56 @@ constexpr int kReadRows = 64;  // positions of one CTA
 
 template <typename T, int D, int CT>
 __global__ void __launch_bounds__(kReadThreads) paged_q8_read_kernel(PagedQ8Read kp) {
-  constexpr int L = D / 8, PER = kReadThreads / L;  // lanes of a row; rows of a pass
+  // 16 codes a load; K and V of a position are two rows of the list
+  constexpr int L = D / 16, PER = kReadThreads / L, N = 2 * kReadRows / PER;
+  __shared__ int row_s[kReadRows];
+  __shared__ float scale_s[2][kReadRows];
   pdl_wait();
   pdl_trigger();
   const int h = blockIdx.y, b = blockIdx.z;
   const int64_t t0 = (int64_t)blockIdx.x * kReadRows;
-  const int n = __ldg(kp.lens + b), lane = threadIdx.x & (L - 1);
-  if (threadIdx.x == 0 && t0 == 0 && h == 0 && (n < 0 || n > kp.cap)) report_device_error(kp.err, kErrPagedQ8, b);
-  bool bad = false;
-  for (int64_t t = t0 + threadIdx.x / L; t < t0 + kReadRows && t < kp.cap; t += PER) {
-    const int row = t < n ? q8_row(kp.bt, kp.maxb, kp.nblocks, kp.bs, kp.HK, b, h, (int)t) : -1;
-    bad |= t < n && row < 0;
-    const size_t o = (((size_t)b * kp.HK + h) * kp.cap + t) * D + lane * 8;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      alignas(16) T y[8];
-      uint2 w = make_uint2(0, 0);
-      float scale = 0.f;
-      if (row >= 0) {
-        w = __ldg(reinterpret_cast<const uint2*>((s ? kp.vc : kp.kc) + (size_t)row * D) + lane);
-        scale = __ldg((s ? kp.vscale : kp.kscale) + row);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        y[e] = from_f<T>(row >= 0 ? value_of<CT>(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xffu) * scale : 0.f);
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(s ? kp.v : kp.k) + o);
-#pragma unroll
-      for (int u = 0; u < (int)sizeof(T) / 2; ++u) dst[u] = reinterpret_cast<const uint4*>(y)[u];
-    }
+  const int n = __ldg(kp.lens + b);
+  if ((int)threadIdx.x < kReadRows) {
+    const int64_t t = t0 + threadIdx.x;
+    if (t == 0 && h == 0 && (n < 0 || n > kp.cap)) report_device_error(kp.err, kErrPagedQ8, b);
+    const bool in = t < n && t < kp.cap;
+    const int row = in ? q8_row(kp.bt, kp.maxb, kp.nblocks, kp.bs, kp.HK, b, h, (int)t) : -1;
+    if (in && row < 0) report_device_error(kp.err, kErrPagedQ8, b);
+    row_s[threadIdx.x] = row;
+    scale_s[0][threadIdx.x] = row < 0 ? 0.f : __ldg(kp.kscale + row);
+    scale_s[1][threadIdx.x] = row < 0 ? 0.f : __ldg(kp.vscale + row);
   }
-  if (bad && lane == 0) report_device_error(kp.err, kErrPagedQ8, b);
+  __syncthreads();
+  const int lane = threadIdx.x & (L - 1);
+  uint4 w[N];
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const int r = u * PER + (int)threadIdx.x / L, s = r / kReadRows, row = row_s[r % kReadRows];
+    w[u] = row < 0 ? make_uint4(0, 0, 0, 0)
+                   : ld_stream_u4((s ? kp.vc : kp.kc) + (size_t)row * D + lane * 16);
+  }
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const int r = u * PER + (int)threadIdx.x / L, s = r / kReadRows, i = r % kReadRows;
+    if (t0 + i >= kp.cap) continue;
+    const float scale = scale_s[s][i];
+    const bool zero = row_s[i] < 0;
+    alignas(16) T y[16];
+    const uint32_t c[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t h01, h23;
+      widen<CT>(c[q], h01, h23);
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h01));
+      const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&h23));
+      y[4 * q] = from_f<T>(zero ? 0.f : a.x * scale), y[4 * q + 1] = from_f<T>(zero ? 0.f : a.y * scale);
+      y[4 * q + 2] = from_f<T>(zero ? 0.f : d.x * scale), y[4 * q + 3] = from_f<T>(zero ? 0.f : d.y * scale);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(s ? kp.v : kp.k) +
+                                          (((size_t)b * kp.HK + h) * kp.cap + t0 + i) * D + lane * 16);
+#pragma unroll
+    for (int q = 0; q < (int)sizeof(T); ++q) dst[q] = reinterpret_cast<const uint4*>(y)[q];
+  }
 }
 
 bool aligned16(const void* p, int64_t stride_bytes) {
@@ -216,8 +293,16 @@ template <typename T, int D, int CT>
 cudaError_t write_t(const PagedQ8& a, cudaStream_t st) {
   const int es = (int)sizeof(T);
   int vec = aligned16(a.k, a.ks * es) && aligned16(a.v, a.vs * es) ? 1 : 0;
-  if (a.rot && aligned16(a.cos_c, (int64_t)a.half * es) && aligned16(a.sin_c, (int64_t)a.half * es)) vec |= 2;
-  return launch_k(paged_q8_write_kernel<T, D, CT>, dim3((unsigned)a.ntok), dim3(kWriteThreads), 0, st, a, vec);
+  if (a.rot && !a.inter && a.half % 8 == 0 && aligned16(a.cos_c, (int64_t)a.half * es) && aligned16(a.sin_c, 0)) vec |= 2;
+  // four rows a thread keep enough loads in flight; one where that would leave SMs without a CTA (5 tokens: 8.3 us
+  // with four, 4.2 us with one)
+  constexpr int per = kWriteThreads / (D / 8);
+  const int64_t rows = (int64_t)a.ntok * 2 * a.HK;
+  if (rows >= (int64_t)per * 4 * num_sms())
+    return launch_k(paged_q8_write_kernel<T, D, CT, 4>, dim3((unsigned)div_up(rows, 4 * per)), dim3(kWriteThreads), 0,
+                    st, a, vec);
+  return launch_k(paged_q8_write_kernel<T, D, CT, 1>, dim3((unsigned)div_up(rows, per)), dim3(kWriteThreads), 0, st, a,
+                  vec);
 }
 
 template <typename T, int D, int CT>

@@ -25,8 +25,6 @@
 //     parts in the order of the keys, so results do not depend on timing.
 // A row whose position lies outside the block table or the cos / sin rows, or that no sequence owns, gives zeros; a key
 // whose page lies outside the tables is skipped; both set the device error word.
-#include <cuda_fp8.h>
-
 #include <algorithm>
 #include <type_traits>
 
@@ -92,24 +90,6 @@ template <int D>
 __host__ __device__ __forceinline__ constexpr int vbyte(int g, int w) {
   if (D == 256) return (w >> 2) * 128 + g * 16 + (w & 3) * 4;
   return g * (D / 8) + w * 4;
-}
-
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
-
-// The four codes of a word as two f16x2 (codes 0, 1 and 2, 3).
-template <int CT>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t& h01, uint32_t& h23) {
-  if constexpr (CT == kI8) {
-    // 0x6400 | (code + 128) is 1024 + 128 + code in fp16
-    const uint32_t x = w ^ 0x80808080u;
-    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    uint32_t a = prmt(x, 0x64646464u, 0x4140), b = prmt(x, 0x64646464u, 0x4342);
-    __half2 ha = __hsub2(*reinterpret_cast<__half2*>(&a), bias), hb = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
-    h01 = *reinterpret_cast<uint32_t*>(&ha), h23 = *reinterpret_cast<uint32_t*>(&hb);
-  } else {
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
-        : "=r"(h01), "=r"(h23) : "r"(w));
-  }
 }
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {

@@ -21,6 +21,8 @@ int check_geometry(const b200ep_paged_q8_params* p, int dtype, const char* op) {
                    n + ": head_size must be 32, 64, 128 or 256");
   B200EP_CHECK_ARG(p->batch >= 0 && p->num_tokens >= 0 && p->kv_heads > 0 && p->kv_heads <= 65535,
                    n + ": batch, num_tokens >= 0 and 0 < kv_heads < 65536 required");
+  B200EP_CHECK_ARG((int64_t)p->num_tokens * 2 * p->kv_heads < (1ll << 31),
+                   n + ": num_tokens * kv_heads must be below 2^30");
   B200EP_CHECK_ARG(p->num_tokens == 0 || p->batch > 0, n + ": packed rows need a sequence to belong to");
   B200EP_CHECK_ARG(p->num_blocks > 0 && p->block_size > 0 && p->max_blocks > 0 &&
                        (int64_t)p->num_blocks * p->block_size < (1ll << 31) &&
