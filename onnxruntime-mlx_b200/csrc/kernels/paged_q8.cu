@@ -66,21 +66,28 @@ __device__ __forceinline__ void rope8(float (&x)[8], const T* row, int d0, const
   }
 }
 
-// x F / amax to codes, 8 of them.  The quick quotient x r, r = F / amax, is within 2^-22 of the true one: where that
-// cannot move any of them over a rounding point it decides, else the division does.  Adding 1.5 2^23 rounds to a whole
-// number whose low byte is the code (the conversion instructions run at an eighth of the rate).
+// The larger of two numbers, a NaN if either is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// x F / amax to codes, 8 of them.  With r = F / amax to two last places, x r is within 2^-21 of the true quotient:
+// where that cannot move any of them over a rounding point it decides, else the division does.  Adding 1.5 2^23
+// rounds to a whole number whose low byte is the code (the conversion instructions run at an eighth of the rate).
 template <int CT>
-__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float amax, float r) {
+__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float amax) {
   uint32_t w[2];
   bool near_tie = false;
+  const float r = __fdividef(CT == kI8 ? 127.f : 448.f, amax);
   if constexpr (CT == kI8) {
     constexpr float kMagic = 12582912.f;
     float y[8], off = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float t = __fmul_rn(x[e], r);
-      y[e] = __fadd_rn(t, kMagic);
-      off = fmaxf(off, fabsf(__fsub_rn(t, __fsub_rn(y[e], kMagic))));
+      y[e] = fmaf(x[e], r, kMagic);
+      off = fmaxf(off, fabsf(fmaf(x[e], r, kMagic - y[e])));
     }
     near_tie = !(off < 0.4999f);
     if (near_tie)
@@ -92,13 +99,13 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], float amax, float
       w[q] = prmt(prmt(b[0], b[1], 0x0040), prmt(b[2], b[3], 0x0040), 0x5410);
     }
   } else {
+    const float lo = r * 0.9999995f, hi = r * 1.0000005f;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const float2 t = make_float2(__fmul_rn(x[e], r), __fmul_rn(x[e + 1], r));
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t.x * 0.9999995f, t.y * 0.9999995f), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t.x * 1.0000005f, t.y * 1.0000005f), __NV_SATFINITE, __NV_E4M3);
-      near_tie |= lo != hi;
-      w[e >> 2] = e & 2 ? prmt(w[e >> 2], lo, 0x5410) : lo;
+      const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(x[e] * lo, x[e + 1] * lo), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(x[e] * hi, x[e + 1] * hi), __NV_SATFINITE, __NV_E4M3);
+      near_tie |= a != b;
+      w[e >> 2] = e & 2 ? prmt(w[e >> 2], a, 0x5410) : a;
     }
     if (near_tie)
 #pragma unroll
@@ -133,12 +140,22 @@ __global__ void __launch_bounds__(kWriteThreads) paged_q8_write_kernel(PagedQ8 k
   const int lane = threadIdx.x & (L - 1), d0 = lane * 8;
   uint4 raw[U][VB];
   int tok[U], head[U];  // token (from `first`; -1: past the end); key head, or HK + value head
+  const int step_i = PER / hk2, step_h = PER - step_i * hk2;  // from one of the thread's rows to the next
+  uint32_t r = r0 + threadIdx.x / L;
+  int i = (int)(r / hk2), hd = (int)(r - i * hk2);
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t r = r0 + u * PER + threadIdx.x / L;
-    const int i = r < total ? (int)(r / hk2) : 0;
+  for (int u = 0; u < U; ++u, r += PER) {
+    if (u) {
+      i += step_i, hd += step_h;
+      if (hd >= (int)hk2) hd -= hk2, ++i;
+    }
     tok[u] = r < total ? i - first : -1;
-    head[u] = r < total ? (int)(r - i * hk2) : 0;
+    head[u] = hd;
+    if (r >= total) {
+#pragma unroll
+      for (int w = 0; w < VB; ++w) raw[u][w] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
     const bool is_k = head[u] < kp.HK;
     const T* src = (is_k ? static_cast<const T*>(kp.k) + (size_t)i * kp.ks + (size_t)head[u] * D
                          : static_cast<const T*>(kp.v) + (size_t)i * kp.vs + (size_t)(head[u] - kp.HK) * D) + d0;
@@ -193,35 +210,37 @@ __global__ void __launch_bounds__(kWriteThreads) paged_q8_write_kernel(PagedQ8 k
       if (__any_sync(0xffffffffu, is_k && at.x >= 0)) {
         const int step = kp.half / 8, from = !turned ? lane : lower ? lane + step : lane - step;
         const T *c = reinterpret_cast<const T*>(cs[u]), *s = reinterpret_cast<const T*>(sn[u]);
+        float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          // (both of a pair exchange before either is replaced: element e of all lanes at once)
-          const float y = __shfl_sync(0xffffffffu, x[e], from, L);
-          if (is_k && turned && at.x >= 0) {
-            const float a = __fmul_rn(x[e], to_f<T>(c[e])), b = __fmul_rn(y, to_f<T>(s[e]));
-            x[e] = lower ? __fsub_rn(a, b) : __fadd_rn(a, b);
+        for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], from, L);
+        if (is_k && turned && at.x >= 0)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float a = __fmul_rn(x[e], to_f<T>(c[e])), b = __fmul_rn(y[e], to_f<T>(s[e]));
+            x[e] = __fadd_rn(a, lower ? -b : b);
           }
-        }
       }
     } else if (kp.rot && is_k && at.x >= 0) {
       rope8<T, D>(x, static_cast<const T*>(kp.k) + (size_t)(first + tok[u]) * kp.ks + (size_t)h * D, d0, kp, at.y);
     }
-    uint32_t m = 0;  // |x| as bits: ordered like the values, a NaN above all
+    float amax = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
+    for (int e = 0; e < 8; ++e) amax = max_nan(amax, fabsf(x[e]));
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = L / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (at.x < 0) continue;
-    float amax = __uint_as_float(m), scale = __fdiv_rn(amax, F);
-    if (m >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u);
-    if (amax > 1e30f || amax < 1e-30f) {  // x F and F / amax stay in range (a power of two: exact)
+    float scale = __fdiv_rn(amax, F);
+    uint2 w = make_uint2(0, 0);
+    if (amax > 1e-30f && amax < 1e30f) {
+      w = codes_of<CT>(x, amax);
+    } else if (!(amax < INFINITY)) {
+      scale = __uint_as_float(0x7fc00000u);
+    } else if (amax > 0.f) {  // x F and F / amax stay in range (a power of two: exact)
       const float s = amax > 1.f ? 0x1p-32f : 0x1p64f;
-      amax *= s;
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= s;
+      w = codes_of<CT>(x, amax * s);
     }
-    uint2 w = make_uint2(0, 0);
-    if (m && m < 0x7f800000u) w = codes_of<CT>(x, amax, __fdiv_rn(F, amax));
     const int64_t row = at.x + (int64_t)h * kp.bs;
     *reinterpret_cast<uint2*>((is_k ? kp.kc : kp.vc) + row * D + d0) = w;
     if (lane == 0) (is_k ? kp.kscale : kp.vscale)[row] = scale;
