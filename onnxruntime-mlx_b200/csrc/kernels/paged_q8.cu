@@ -121,130 +121,103 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], float amax) {
 
 constexpr int kWriteThreads = 256;
 
-// The rows of all tokens as one list (the HK key rows of a token, then its HK value rows), kWriteThreads / (D / 8)
-// x U of them a CTA: the page rows of a CTA's tokens are looked up once, and each thread has all its
-// loads on their way before it uses the first.
-template <typename T, int D, int CT, int U>
-__global__ void __launch_bounds__(kWriteThreads) paged_q8_write_kernel(PagedQ8 kp, int vec) {
-  constexpr int L = D / 8, PER = kWriteThreads / L, ROWS = PER * U;  // lanes of a row; rows
+// The rows of all tokens as one list (the HK key rows of a token, then its HK value rows), one to D / 8 lanes.  The
+// page rows of a CTA's tokens are looked up once, while its loads are on their way.  Instructions bound it (about 30
+// an element: two kinds of row, RoPE, the maximum, the rounding), so more rows a thread (2 or 4, measured) only
+// cost occupancy: 32768 tokens of 8 kv heads, head size 128, fp16: 91 us with one, 99 and 103 us with two and four.
+template <typename T, int D, int CT>
+__global__ void __launch_bounds__(kWriteThreads, sizeof(T) == 2 ? 8 : 6) paged_q8_write_kernel(PagedQ8 kp, int vec) {
+  constexpr int L = D / 8, ROWS = kWriteThreads / L;  // lanes of a row; rows
   constexpr float F = CT == kI8 ? 127.f : 448.f;
-  constexpr int VB = sizeof(T) / 2;  // 16-byte loads of 8 elements
-  __shared__ int2 tok_s[ROWS];       // a token's page row (-1: none) and position
+  __shared__ int2 tok_s[ROWS];  // a token's page row (-1: none) and position
   pdl_wait();
   pdl_trigger();
   if (kp.counters && blockIdx.x == 0)  // the attention launch that follows counts arrivals from zero
     for (int t = threadIdx.x; t < kp.ctas; t += kWriteThreads) kp.counters[t] = 0;
   const uint32_t r0 = blockIdx.x * ROWS, total = (uint32_t)kp.ntok * 2 * kp.HK, hk2 = 2 * kp.HK;  // (below 2^31)
-  const int first = (int)(r0 / hk2);
-  const int ntok = (int)((min(total, r0 + ROWS) - 1) / hk2) - first + 1;
+  const int first = (int)(r0 / hk2), ntok = (int)((min(total, r0 + ROWS) - 1) / hk2) - first + 1;
   const int lane = threadIdx.x & (L - 1), d0 = lane * 8;
-  uint4 raw[U][VB];
-  int tok[U], head[U];  // token (from `first`; -1: past the end); key head, or HK + value head
-  const int step_i = PER / hk2, step_h = PER - step_i * hk2;  // from one of the thread's rows to the next
-  uint32_t r = r0 + threadIdx.x / L;
-  int i = (int)(r / hk2), hd = (int)(r - i * hk2);
+  const uint32_t r = r0 + threadIdx.x / L;
+  const bool live = r < total;
+  const int i = (int)((live ? r : r0) / hk2), hd = (int)((live ? r : r0) - i * hk2);
+  const bool is_k = hd < kp.HK;
+  const int h = is_k ? hd : hd - kp.HK;
+  const T* src = (is_k ? static_cast<const T*>(kp.k) + (size_t)i * kp.ks : static_cast<const T*>(kp.v) + (size_t)i * kp.vs) +
+                 (size_t)h * D;
+  uint4 raw[sizeof(T) / 2];
+  if (vec & 1) {
 #pragma unroll
-  for (int u = 0; u < U; ++u, r += PER) {
-    if (u) {
-      i += step_i, hd += step_h;
-      if (hd >= (int)hk2) hd -= hk2, ++i;
-    }
-    tok[u] = r < total ? i - first : -1;
-    head[u] = hd;
-    if (r >= total) {
+    for (int w = 0; w < (int)sizeof(T) / 2; ++w) raw[w] = __ldg(reinterpret_cast<const uint4*>(src + d0) + w);
+  } else {
 #pragma unroll
-      for (int w = 0; w < VB; ++w) raw[u][w] = make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    const bool is_k = head[u] < kp.HK;
-    const T* src = (is_k ? static_cast<const T*>(kp.k) + (size_t)i * kp.ks + (size_t)head[u] * D
-                         : static_cast<const T*>(kp.v) + (size_t)i * kp.vs + (size_t)(head[u] - kp.HK) * D) + d0;
-    if (vec & 1) {
-#pragma unroll
-      for (int w = 0; w < VB; ++w) raw[u][w] = __ldg(reinterpret_cast<const uint4*>(src) + w);
-    } else {
-      T* e = reinterpret_cast<T*>(raw[u]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = src[j];
-    }
+    for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(raw)[e] = src[d0 + e];
   }
-  if ((int)threadIdx.x < ntok) {
-    const int i = first + threadIdx.x;
-    const int b = q8_seq(kp.cum, kp.batch, i);
-    const int pos = b >= 0 ? __ldg(kp.past + b) + (i - __ldg(kp.cum + b)) : -1;
-    const bool ok = pos >= 0 && !(kp.rot && pos >= kp.max_seq);
-    const int row = ok ? q8_row(kp.bt, kp.maxb, kp.nblocks, kp.bs, kp.HK, b, 0, pos) : -1;
-    if (row < 0) report_device_error(kp.err, kErrPagedQ8, i);
-    tok_s[threadIdx.x] = make_int2(row, pos);
+  // a warp a token: the sequence is the number of sequences that end at or before the row (one look at 32 ends at once,
+  // where a search would wait for each of its steps)
+  for (int q = threadIdx.x >> 5; q < ntok; q += kWriteThreads / 32) {
+    const int t = first + q, ln = threadIdx.x & 31;
+    int b = 0;
+    for (int b0 = 0; b0 < kp.batch; b0 += 32) {
+      const bool ends = b0 + ln < kp.batch && __ldg(kp.cum + b0 + ln + 1) <= t;
+      const int n = __popc(__ballot_sync(0xffffffffu, ends));
+      b += n;
+      if (n < 32) break;
+    }
+    if (ln) continue;
+    int pos = -1, row = -1;
+    if (b < kp.batch) pos = __ldg(kp.past + b) + (t - __ldg(kp.cum + b));
+    if (t >= __ldg(kp.cum) && pos >= 0 && !(kp.rot && pos >= kp.max_seq))
+      row = q8_row(kp.bt, kp.maxb, kp.nblocks, kp.bs, kp.HK, b, 0, pos);
+    if (row < 0) report_device_error(kp.err, kErrPagedQ8, t);
+    tok_s[q] = make_int2(row, pos);
   }
   __syncthreads();
-  // halves of whole 8-element chunks, aligned rows: the partner's elements are another lane's, and the angles of
-  // all rows are on their way before the first is used
-  const bool wide = kp.rot && (vec & 2);
-  const bool turned = d0 < 2 * kp.half, lower = d0 < kp.half;
-  uint4 cs[U][VB], sn[U][VB];
-  if (wide && turned)
+  const int2 at = live ? tok_s[i - first] : make_int2(-1, 0);
+  const bool turn = kp.rot && is_k && at.x >= 0;
+  float x[8];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int pos = tok[u] >= 0 && tok_s[tok[u]].x >= 0 ? tok_s[tok[u]].y : -1;
-      if (pos < 0 || head[u] >= kp.HK) continue;
-      const size_t o = (size_t)pos * kp.half + (lower ? d0 : d0 - kp.half);
+  for (int e = 0; e < 8; ++e) x[e] = to_f<T>(reinterpret_cast<const T*>(raw)[e]);
+  if ((vec & 2) && __any_sync(0xffffffffu, turn)) {  // halves of whole 8-element chunks, aligned rows: the partner's elements are another lane's
+    const bool turned = d0 < 2 * kp.half, lower = d0 < kp.half;
+    const int step = kp.half / 8, from = !turned ? lane : lower ? lane + step : lane - step;
+    float y[8];
 #pragma unroll
-      for (int w = 0; w < VB; ++w) {
-        cs[u][w] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(kp.cos_c) + o) + w);
-        sn[u][w] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(kp.sin_c) + o) + w);
+    for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], from, L);
+    if (turn && turned) {
+      const size_t o = (size_t)at.y * kp.half + (lower ? d0 : d0 - kp.half);
+      float c[8], s[8];
+      load8<T>(static_cast<const T*>(kp.cos_c) + o, true, c);
+      load8<T>(static_cast<const T*>(kp.sin_c) + o, true, s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = __fmul_rn(x[e], c[e]), b = __fmul_rn(y[e], s[e]);
+        x[e] = __fadd_rn(a, lower ? -b : b);
       }
     }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {  // (all lanes of a warp take part in the shuffles)
-    const int2 at = tok[u] >= 0 ? tok_s[tok[u]] : make_int2(-1, 0);
-    const bool is_k = head[u] < kp.HK;
-    const int h = is_k ? head[u] : head[u] - kp.HK;
-    float x[8];
-    {
-      const T* e = reinterpret_cast<const T*>(raw[u]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = to_f<T>(e[j]);
-    }
-    if (wide) {
-      if (__any_sync(0xffffffffu, is_k && at.x >= 0)) {
-        const int step = kp.half / 8, from = !turned ? lane : lower ? lane + step : lane - step;
-        const T *c = reinterpret_cast<const T*>(cs[u]), *s = reinterpret_cast<const T*>(sn[u]);
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], from, L);
-        if (is_k && turned && at.x >= 0)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float a = __fmul_rn(x[e], to_f<T>(c[e])), b = __fmul_rn(y[e], to_f<T>(s[e]));
-            x[e] = __fadd_rn(a, lower ? -b : b);
-          }
-      }
-    } else if (kp.rot && is_k && at.x >= 0) {
-      rope8<T, D>(x, static_cast<const T*>(kp.k) + (size_t)(first + tok[u]) * kp.ks + (size_t)h * D, d0, kp, at.y);
-    }
-    float amax = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) amax = max_nan(amax, fabsf(x[e]));
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (at.x < 0) continue;
-    float scale = __fdiv_rn(amax, F);
-    uint2 w = make_uint2(0, 0);
-    if (amax > 1e-30f && amax < 1e30f) {
-      w = codes_of<CT>(x, amax);
-    } else if (!(amax < INFINITY)) {
-      scale = __uint_as_float(0x7fc00000u);
-    } else if (amax > 0.f) {  // x F and F / amax stay in range (a power of two: exact)
-      const float s = amax > 1.f ? 0x1p-32f : 0x1p64f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= s;
-      w = codes_of<CT>(x, amax * s);
-    }
-    const int64_t row = at.x + (int64_t)h * kp.bs;
-    *reinterpret_cast<uint2*>((is_k ? kp.kc : kp.vc) + row * D + d0) = w;
-    if (lane == 0) (is_k ? kp.kscale : kp.vscale)[row] = scale;
+  } else if (turn) {
+    rope8<T, D>(x, src, d0, kp, at.y);
   }
+  float amax = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) amax = max_nan(amax, fabsf(x[e]));
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if (at.x < 0) return;
+  float scale = __fdiv_rn(amax, F);
+  uint2 w = make_uint2(0, 0);
+  if (amax > 1e-30f && amax < 1e30f) {
+    w = codes_of<CT>(x, amax);
+  } else if (!(amax < INFINITY)) {
+    scale = __uint_as_float(0x7fc00000u);
+  } else if (amax > 0.f) {  // x F and F / amax stay in range (a power of two: exact)
+    const float s = amax > 1.f ? 0x1p-32f : 0x1p64f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= s;
+    w = codes_of<CT>(x, amax * s);
+  }
+  const int64_t row = at.x + (int64_t)h * kp.bs;
+  *reinterpret_cast<uint2*>((is_k ? kp.kc : kp.vc) + row * D + d0) = w;
+  if (lane == 0) (is_k ? kp.kscale : kp.vscale)[row] = scale;
 }
 
 constexpr int kReadThreads = 256;
@@ -313,15 +286,9 @@ cudaError_t write_t(const PagedQ8& a, cudaStream_t st) {
   const int es = (int)sizeof(T);
   int vec = aligned16(a.k, a.ks * es) && aligned16(a.v, a.vs * es) ? 1 : 0;
   if (a.rot && !a.inter && a.half % 8 == 0 && aligned16(a.cos_c, (int64_t)a.half * es) && aligned16(a.sin_c, 0)) vec |= 2;
-  // four rows a thread keep enough loads in flight; one where that would leave SMs without a CTA (5 tokens: 8.3 us
-  // with four, 4.2 us with one)
-  constexpr int per = kWriteThreads / (D / 8);
-  const int64_t rows = (int64_t)a.ntok * 2 * a.HK;
-  if (rows >= (int64_t)per * 4 * num_sms())
-    return launch_k(paged_q8_write_kernel<T, D, CT, 4>, dim3((unsigned)div_up(rows, 4 * per)), dim3(kWriteThreads), 0,
-                    st, a, vec);
-  return launch_k(paged_q8_write_kernel<T, D, CT, 1>, dim3((unsigned)div_up(rows, per)), dim3(kWriteThreads), 0, st, a,
-                  vec);
+  constexpr int rows = kWriteThreads / (D / 8);
+  return launch_k(paged_q8_write_kernel<T, D, CT>, dim3((unsigned)div_up((int64_t)a.ntok * 2 * a.HK, rows)),
+                  dim3(kWriteThreads), 0, st, a, vec);
 }
 
 template <typename T, int D, int CT>
