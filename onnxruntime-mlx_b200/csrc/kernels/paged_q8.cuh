@@ -24,7 +24,7 @@ struct PagedQ8 {
   const void *cos_c, *sin_c;
   void* out;
   DeviceErrorSlot* err;
-  int batch, ntok, H, HK, D, G, nblocks, bs, maxb, max_seq, half, rot, inter;
+  int batch, ntok, H, HK, D, G, nblocks, bs, bs_shift, maxb, max_seq, half, rot, inter;
   int dtype, ctype;
   float scale;
   // attention work split (see paged_q8_attn.cu)
@@ -57,9 +57,11 @@ __device__ __forceinline__ int q8_seq(const int32_t* cum, int batch, int i) {
   return lo;
 }
 
-// Row (of block_size-row pages of one kv head) of position pos of sequence b for kv head h, or -1.
-__device__ __forceinline__ int q8_row(const int32_t* bt, int maxb, int nblocks, int bs, int HK, int b, int h, int pos) {
-  const int blk = pos / bs;
+// Row (of block_size-row pages of one kv head) of position pos of sequence b for kv head h, or -1.  shift: log2 of
+// the block size where that is a power of two, else -1.
+__device__ __forceinline__ int q8_row(const int32_t* bt, int maxb, int nblocks, int bs, int HK, int b, int h, int pos,
+                                      int shift = -1) {
+  const int blk = shift >= 0 ? pos >> shift : pos / bs;
   if (pos < 0 || blk >= maxb) return -1;
   const int phys = __ldg(bt + (size_t)b * maxb + blk);
   return phys < 0 || phys >= nblocks ? -1 : (phys * HK + h) * bs + (pos - blk * bs);

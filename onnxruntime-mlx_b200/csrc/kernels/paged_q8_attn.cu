@@ -37,6 +37,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRowTab = 64;
 constexpr int kLift = 6;       // P vs is held times 2^kLift
+constexpr float kLow = -1e30f;  // the running maximum before the first key: far below any, and finite
 constexpr float kSlack = 8.f;  // a score may pass the running maximum by this much (in base 2) before it moves
 
 template <typename T, int D, int CT, int NT>
@@ -367,7 +368,8 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
     if (ix >= run) return -1;
     const int key = is.u * U + (paged ? 0 : lane);
     return key < is.n && (paged || lane < U)
-               ? q8_row(kp.bt, kp.maxb, kp.nblocks, kp.bs, kp.HK, is.seq, hchunks == 1 ? is.hc : is.hc / hchunks, key)
+               ? q8_row(kp.bt, kp.maxb, kp.nblocks, kp.bs, kp.HK, is.seq, hchunks == 1 ? is.hc : is.hc / hchunks, key,
+                        kp.bs_shift)
                : -1;
   };
   int next_row = lookup(warp);
@@ -518,11 +520,14 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       if (vec & 1) fetch_q(nx);
     }
 
+    float qs[NT][2];  // what turns a score's sum into base-2 logits, but for the key's scale
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) qs[nt][0] = qscale[nt * 8 + 2 * c], qs[nt][1] = qscale[nt * 8 + 2 * c + 1];
     float o[MT][NT][4], m[NT][2], l[NT][2];
     int E = kLift + 1;  // biased exponent that P vs is relative to
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
+      m[nt][0] = m[nt][1] = kLow, l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
       for (int t = 0; t < MT; ++t) o[t][nt][0] = o[t][nt][1] = o[t][nt][2] = o[t][nt][3] = 0.f;
     }
@@ -604,7 +609,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
           }
         }
         }
-        // scores in base 2: key g (r = 0) and g + 8 (r = 1), heads 2c and 2c + 1
+        // scores in base 2, key g (r = 0) and g + 8 (r = 1), heads 2c and 2c + 1
         float vs[2];
         bool move = false;
 #pragma unroll
@@ -617,7 +622,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float v = on ? s[nt][r * 2 + h] * (ks * lds_f(smem_u32(qscale) + (nt * 8 + 2 * c + h) * 4)) : -INFINITY;
+              const float v = on ? s[nt][r * 2 + h] * (ks * qs[nt][h]) : -INFINITY;
               s[nt][r * 2 + h] = v;
               move |= v > m[nt][h] + kSlack;
             }
@@ -634,7 +639,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
               float mx = fmaxf(m[nt][h], fmaxf(s[nt][h], s[nt][2 + h]));
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-              const float a = m[nt][h] == -INFINITY ? 0.f : ex2(m[nt][h] - mx);
+              const float a = ex2(m[nt][h] - mx);
               m[nt][h] = mx;
               l[nt][h] *= a;
 #pragma unroll
@@ -651,8 +656,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
             float p[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float v = s[nt][r * 2 + h];
-              p[h] = v == -INFINITY ? 0.f : ex2(v - m[nt][h]);
+              p[h] = ex2(s[nt][r * 2 + h] - m[nt][h]);
               l[nt][h] += p[h];
               p[h] *= vs[r] * down;
             }
@@ -794,24 +798,25 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
             const float a0 = ll == 0.f ? 0.f : ex2(mm - mn);
             mm = mn, ll *= a0;
             acc.x *= a0, acc.y *= a0, acc.z *= a0, acc.w *= a0;
-            const float* pk = part_at(k0) + hd * D + d;
-            constexpr int MLP = 6;  // parts on their way at once
+            auto take = [&](const float4& v, int k) {
+              const float2 ml = mlb[k * C::kHeads + hd];
+              const float f = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
+              ll += ml.y * f;
+              acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+            };
+            int k = 0;
+            if (k0 == 0) take(__ldcg(reinterpret_cast<const float4*>(part_at(0) + hd * D + d)), k++);
+            const float* pk = first + (k0 + k) * step + hd * D + d;
+            constexpr int MLP = 8;  // parts on their way at once
 #pragma unroll 1
-            for (int k = 0; k < nk; k += MLP) {
+            for (; k < nk; k += MLP, pk += MLP * step) {
               float4 v[MLP];
 #pragma unroll
-              for (int j = 0; j < MLP; ++j) {
-                if (k + j < nk) v[j] = __ldcg(reinterpret_cast<const float4*>(pk));
-                pk += k0 + k + j ? step : step / 2;
-              }
+              for (int j = 0; j < MLP; ++j)
+                if (k + j < nk) v[j] = __ldcg(reinterpret_cast<const float4*>(pk + j * step));
 #pragma unroll
-              for (int j = 0; j < MLP; ++j) {
-                if (k + j >= nk) break;
-                const float2 ml = mlb[(k + j) * C::kHeads + hd];
-                const float f = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
-                ll += ml.y * f;
-                acc.x += v[j].x * f, acc.y += v[j].y * f, acc.z += v[j].z * f, acc.w += v[j].w * f;
-              }
+              for (int j = 0; j < MLP; ++j)
+                if (k + j < nk) take(v[j], k + j);
             }
           }
           if (on) store4<T>(out + hd * D + d, acc, ll);

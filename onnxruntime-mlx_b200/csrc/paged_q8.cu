@@ -44,6 +44,9 @@ PagedQ8 common(const b200ep_paged_q8_params* p, void* kc, void* vc, float* ks, f
   a.cum = cum, a.past = past, a.bt = bt, a.cos_c = cos_c, a.sin_c = sin_c, a.err = device_error_slot();
   a.batch = p->batch, a.ntok = p->num_tokens, a.H = p->num_heads, a.HK = p->kv_heads, a.D = p->head_size;
   a.nblocks = p->num_blocks, a.bs = p->block_size, a.maxb = p->max_blocks, a.max_seq = p->max_seq;
+  a.bs_shift = -1;
+  for (int t = 0; t < 31; ++t)
+    if (a.bs == 1 << t) a.bs_shift = t;
   a.half = p->rotary_half, a.rot = p->do_rotary ? 1 : 0, a.inter = p->interleaved ? 1 : 0;
   a.dtype = dtype, a.ctype = p->cache_type;
   a.ks = p->key_stride ? p->key_stride : (int64_t)p->kv_heads * p->head_size;
