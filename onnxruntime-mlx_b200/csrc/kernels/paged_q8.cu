@@ -17,6 +17,7 @@
 
 #include <cuda_fp8.h>
 
+#include <cstring>
 #include <type_traits>
 
 namespace b200ep {
@@ -29,7 +30,8 @@ __device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
     uint4 w[sizeof(T) / 2];
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    const T* h = reinterpret_cast<const T*>(w);
+    T h[8];
+    memcpy(h, w, sizeof(h));
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = to_f<T>(h[e]);
   } else {
@@ -95,8 +97,8 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], float amax) {
       for (int e = 0; e < 8; ++e) y[e] = __fadd_rn(__fdiv_rn(__fmul_rn(x[e], 127.f), amax), kMagic);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const uint32_t* b = reinterpret_cast<const uint32_t*>(y + 4 * q);
-      w[q] = prmt(prmt(b[0], b[1], 0x0040), prmt(b[2], b[3], 0x0040), 0x5410);
+      w[q] = prmt(prmt(__float_as_uint(y[4 * q]), __float_as_uint(y[4 * q + 1]), 0x0040),
+                  prmt(__float_as_uint(y[4 * q + 2]), __float_as_uint(y[4 * q + 3]), 0x0040), 0x5410);
     }
   } else {
     const float lo = r * 0.9999995f, hi = r * 1.0000005f;
@@ -149,8 +151,10 @@ __global__ void __launch_bounds__(kWriteThreads, sizeof(T) == 2 ? 8 : 6) paged_q
 #pragma unroll
     for (int w = 0; w < (int)sizeof(T) / 2; ++w) raw[w] = __ldg(reinterpret_cast<const uint4*>(src + d0) + w);
   } else {
+    T one[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(raw)[e] = src[d0 + e];
+    for (int e = 0; e < 8; ++e) one[e] = src[d0 + e];
+    memcpy(raw, one, sizeof(one));
   }
   // a warp a token: the sequence is the number of sequences that end at or before the row (one look at 32 ends at once,
   // where a search would wait for each of its steps)
@@ -175,8 +179,12 @@ __global__ void __launch_bounds__(kWriteThreads, sizeof(T) == 2 ? 8 : 6) paged_q
   const int2 at = live ? tok_s[i - first] : make_int2(-1, 0);
   const bool turn = kp.rot && is_k && at.x >= 0;
   float x[8];
+  {
+    T one[8];
+    memcpy(one, raw, sizeof(one));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = to_f<T>(reinterpret_cast<const T*>(raw)[e]);
+    for (int e = 0; e < 8; ++e) x[e] = to_f<T>(one[e]);
+  }
   if ((vec & 2) && __any_sync(0xffffffffu, turn)) {  // halves of whole 8-element chunks, aligned rows: the partner's elements are another lane's
     const bool turned = d0 < 2 * kp.half, lower = d0 < kp.half;
     const int step = kp.half / 8, from = !turned ? lane : lower ? lane + step : lane - step;
@@ -273,7 +281,11 @@ __global__ void __launch_bounds__(kReadThreads) paged_q8_read_kernel(PagedQ8Read
     uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(s ? kp.v : kp.k) +
                                           (((size_t)b * kp.HK + h) * kp.cap + t0 + i) * D + lane * 16);
 #pragma unroll
-    for (int q = 0; q < (int)sizeof(T); ++q) dst[q] = reinterpret_cast<const uint4*>(y)[q];
+    for (int q = 0; q < (int)sizeof(T); ++q) {
+      uint4 b;
+      memcpy(&b, y + q * (16 / sizeof(T)), 16);
+      dst[q] = b;
+    }
   }
 }
 

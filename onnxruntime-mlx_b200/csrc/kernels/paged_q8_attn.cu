@@ -26,6 +26,7 @@
 // A row whose position lies outside the block table or the cos / sin rows, or that no sequence owns, gives zeros; a key
 // whose page lies outside the tables is skipped; both set the device error word.
 #include <algorithm>
+#include <cstring>
 #include <type_traits>
 
 #include "paged_q8.cuh"
@@ -184,8 +185,10 @@ template <typename T>
 __device__ __forceinline__ void store4(T* dst, float4 a, float l) {
   const float r = l == 0.f ? 0.f : __frcp_rn(l);
   alignas(4 * sizeof(T)) T v[4] = {from_f<T>(a.x * r), from_f<T>(a.y * r), from_f<T>(a.z * r), from_f<T>(a.w * r)};
-  if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(v);
-  else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+  using W = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
+  W w;
+  memcpy(&w, v, sizeof(w));
+  *reinterpret_cast<W*>(dst) = w;
 }
 
 template <typename T, int D, int CT, int NT>

@@ -27,6 +27,7 @@
 #include <cooperative_groups.h>
 
 #include <cmath>
+#include <cstring>
 
 #include "../common.cuh"
 #include "sample.h"
@@ -105,13 +106,16 @@ struct Vec;
 template <>
 struct Vec<float> {
   static __device__ __forceinline__ float clean(uint4& w) {
-    float* f = reinterpret_cast<float*>(&w);
+    float f[4];
+    memcpy(f, &w, 16);
 #pragma unroll
     for (int j = 0; j < 4; ++j) f[j] = fmaxf(f[j], -INFINITY);
+    memcpy(&w, f, 16);
     return largest(w);
   }
   static __device__ __forceinline__ float largest(const uint4& w) {
-    const float* f = reinterpret_cast<const float*>(&w);
+    float f[4];
+    memcpy(f, &w, 16);
     return fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
   }
 };
@@ -124,13 +128,16 @@ __device__ __forceinline__ __nv_bfloat162 both<__nv_bfloat162>(float v) { return
 template <typename T2>
 struct Vec16 {
   static __device__ __forceinline__ float clean(uint4& w) {
-    T2* h = reinterpret_cast<T2*>(&w);
+    T2 h[4];
+    memcpy(h, &w, 16);
 #pragma unroll
     for (int j = 0; j < 4; ++j) h[j] = __hmax2(h[j], both<T2>(-INFINITY));  // (the operand that is a number)
+    memcpy(&w, h, 16);
     return largest(w);
   }
   static __device__ __forceinline__ float largest(const uint4& w) {
-    const T2* h = reinterpret_cast<const T2*>(&w);
+    T2 h[4];
+    memcpy(h, &w, 16);
     const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
     return fmaxf(to_f(m.x), to_f(m.y));
   }
@@ -210,7 +217,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     for (int i = tid; i < nvec; i += kThreads) {
       const uint4 w = *reinterpret_cast<const uint4*>(stage + i * VE);
       if (Vec<T>::largest(w) < least) continue;
-      const T* v = reinterpret_cast<const T*>(&w);
+      T v[VE];
+      memcpy(v, &w, 16);
 #pragma unroll
       for (int j = 0; j < VE; ++j) f(to_f<T>(v[j]) + 0.f, i * VE + j);  // (-0 and 0 are one value)
     }
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
 
   // ---- top-k from the threads' maxima
   if (k <= kCap && k < a.vocab) {
-    auto bin_of = [&](float v) { return (int)fminf((m - v) * 8.f, (float)(kTop - 1)); };
+    auto bin_of = [&](float v) { return (int)fminf(fmaxf((m - v) * 8.f, 0.f), (float)(kTop - 1)); };
     if (mine > -INFINITY) atomicAdd(&red.top[bin_of(mine)], 1);
     cluster.sync();
     if (warp == 0) {
@@ -472,10 +480,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     for (int b = 0; b < kSplit; ++b) col[b * kThreads + tid] = 0.f;
     {
       uint8_t* mine_col = reinterpret_cast<uint8_t*>(col + tid);
-      auto slot = [&](float v) {  // (2^23's own bits leave the word)
-        return reinterpret_cast<float*>(mine_col + (__float_as_uint(fminf(spot(v), kMagic + (float)(kSplit - 1))) * (uint32_t)(kThreads * 4)));
+      auto slot = [&](float v) {
+        const uint32_t bin = __float_as_uint(fminf(spot(v), kMagic + (float)(kSplit - 1))) & (kSplit - 1);
+        return reinterpret_cast<float*>(mine_col + bin * (kThreads * 4));
       };
-      static_assert(kThreads * 4 >= 512, "the shift of the exponent bits");
       if (by_mass)
         each(-INFINITY, [&](float v, int) { *slot(v) += weight(v); });
       else
@@ -538,7 +546,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       for (int i0 = warp * 32; i0 < nvec; i0 += kThreads) {
         const int i = i0 + lane;
         const uint4 w4 = i < nvec ? *reinterpret_cast<const uint4*>(stage + i * VE) : uint4{};
-        const T* v = reinterpret_cast<const T*>(&w4);
+        T v[VE];
+        memcpy(v, &w4, 16);
         uint32_t in = 0;  // which of the thread's VE tokens
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
@@ -671,11 +680,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     for (int i = tid; i < nvec; i += kThreads) {
       const uint4 w = *reinterpret_cast<const uint4*>(stage + i * VE);
       if (Vec<T>::largest(w) < least) continue;
-      const T* v = reinterpret_cast<const T*>(&w);
-      alignas(16) float en[VE];
+      T v[VE];
+      memcpy(v, &w, 16);
+      float en[VE];
       if (vec && (i + 1) * VE <= n) {
 #pragma unroll
-        for (int q = 0; q < VE / 4; ++q) *reinterpret_cast<uint4*>(en + 4 * q) = ld_stream_u4(e + i * VE + 4 * q);
+        for (int q = 0; q < VE / 4; ++q) {
+          const uint4 b = ld_stream_u4(e + i * VE + 4 * q);
+          en[4 * q] = __uint_as_float(b.x), en[4 * q + 1] = __uint_as_float(b.y);
+          en[4 * q + 2] = __uint_as_float(b.z), en[4 * q + 3] = __uint_as_float(b.w);
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < VE; ++j) en[j] = i * VE + j < n ? __ldg(e + i * VE + j) : 1.f;
