@@ -48,13 +48,13 @@ constexpr int kTop = 128;    // bins of the threads' maxima
 constexpr int kNear = 1024;  // tokens of the border's bin that a warp lists
 static_assert(kSplit == kWarpsS && kCap <= kThreads && kBins <= kThreads, "one warp a bin, one thread a token");
 
-struct Token {
+struct __align__(8) Token {
   float x;
   int index;
 };
 __device__ __forceinline__ bool before(Token a, Token b) { return a.x > b.x || (a.x == b.x && a.index < b.index); }
 
-struct Red {  // what CTAs of a cluster exchange; one slot per use, so that no barrier is needed before reuse
+struct __align__(8) Red {  // what CTAs of a cluster exchange; one slot per use, so that no barrier is needed before reuse
   float maxv, sum;
   unsigned long long mass, best;
   float bin[2][kSplit];  // of the first split, by count and by mass
@@ -144,6 +144,35 @@ struct Vec16 {
 };
 template <> struct Vec<__half> : Vec16<__half2> {};
 template <> struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat162> {};
+
+// Reads and writes of the same variable in CTA r of the cluster.  (As instructions of their own: addresses that the
+// compiler could share over the whole kernel would take up its registers.)
+template <typename V>
+__device__ __forceinline__ V peer(const V* p, int r) {
+  V v;
+  if constexpr (sizeof(V) == 8) {
+    unsigned long long u;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.b64 %0, [a];\n\t}"
+                 : "=l"(u) : "r"(smem_u32(p)), "r"(r) : "memory");
+    memcpy(&v, &u, 8);
+  } else {
+    uint32_t u;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.b32 %0, [a];\n\t}"
+                 : "=r"(u) : "r"(smem_u32(p)), "r"(r) : "memory");
+    memcpy(&v, &u, 4);
+  }
+  return v;
+}
+__device__ __forceinline__ void peer_set(unsigned long long* p, int r, unsigned long long v) {
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tst.shared::cluster.b64 [a], %2;\n\t}" ::"r"(
+                   smem_u32(p)), "r"(r), "l"(v)
+               : "memory");
+}
+__device__ __forceinline__ unsigned long long bits_of(Token t) {
+  unsigned long long u;
+  memcpy(&u, &t, 8);
+  return u;
+}
 
 template <typename V, typename F>
 __device__ __forceinline__ V block_reduce(V v, F f, V* scratch) {
@@ -241,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   cluster.sync();
 #pragma unroll
   for (int r = 0; r < kMaxCluster; ++r)
-    if (r < C) m = fmaxf(m, cluster.map_shared_rank(&red, r)->maxv);
+    if (r < C) m = fmaxf(m, peer(&red.maxv, r));
   m += 0.f;
   if (m == -INFINITY) {  // nothing to choose from
     if (rank == 0 && tid == 0) {
@@ -273,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       float zs = 0.f;
 #pragma unroll
       for (int r = 0; r < kMaxCluster; ++r)
-        if (r < C) zs += cluster.map_shared_rank(&red, r)->sum;
+        if (r < C) zs += peer(&red.sum, r);
       const float v = to_f<T>(static_cast<const T*>(a.logits)[(size_t)row * a.logits_stride + token]);
       a.logprobs[row] = (v == INFINITY ? 0.f : v - m) - logf(zs);
     }
@@ -296,10 +325,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     cluster.sync();
     int c[kMaxCluster], got = 0;
 #pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r) c[r] = r < C ? cluster.map_shared_rank(&red, r)->got : 0;
+    for (int r = 0; r < kMaxCluster; ++r) c[r] = r < C ? peer(&red.got, r) : 0;
 #pragma unroll
     for (int r = 0; r < kMaxCluster; ++r) {
-      if (rank == 0 && tid < c[r] && got + c[r] <= kCap) all[got + tid] = cluster.map_shared_rank(&red, r)->list[tid];
+      if (rank == 0 && tid < c[r] && got + c[r] <= kCap) all[got + tid] = peer(&red.list[tid], r);
       got += c[r];
     }
     __syncthreads();
@@ -361,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
         own[q] = 0;
 #pragma unroll
         for (int r = 0; r < kMaxCluster; ++r)
-          if (r < C) own[q] += cluster.map_shared_rank(&red, r)->top[lane * (kTop / 32) + q];
+          if (r < C) own[q] += peer(&red.top[lane * (kTop / 32) + q], r);
         sum += own[q];
       }
       int inc = sum;
@@ -407,9 +436,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
 #pragma unroll
       for (int r = 0; r < kMaxCluster; ++r)
         if (r < C) {
-          own += cluster.map_shared_rank(cnt, r)[bin];
+          own += peer(cnt + bin, r);
           if (by_mass)
-            val += ((unsigned long long)cluster.map_shared_rank(mhi, r)[bin] << 16) + cluster.map_shared_rank(mlo, r)[bin];
+            val += ((unsigned long long)peer(mhi + bin, r) << 16) + peer(mlo + bin, r);
         }
       if (!by_mass) val = own;
     }
@@ -433,18 +462,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     unsigned long long sum = 0;
 #pragma unroll
     for (int r = 0; r < kMaxCluster; ++r) {
-      const unsigned long long v = r < C ? cluster.map_shared_rank(seg_s, r)[par][0] : 0;
+      const unsigned long long v = r < C ? peer(&seg_s[par][0], r) : 0;
       if (r < rank) ahead_ += v;
       sum += v;
     }
     goal = min(goal, sum);
     if (ahead_ < goal && goal <= ahead_ + val)
       for (int r = 0; r < C; ++r) {
-        auto* f = cluster.map_shared_rank(found_s, r)[par];
-        f[1] = (unsigned)bin;
-        f[2] = ahead_;
-        f[3] = own;
-        f[0] = 1 + (!by_mass && ahead_ + val == goal ? 1 : 0);  // 2: the bin is taken whole
+        unsigned long long* f = found_s[par];
+        peer_set(f + 1, r, (unsigned long long)(unsigned)bin);
+        peer_set(f + 2, r, ahead_);
+        peer_set(f + 3, r, own);
+        peer_set(f, r, !by_mass && ahead_ + val == goal ? 2ull : 1ull);  // 2: the bin is taken whole
       }
     cluster.sync();
     return par;
@@ -504,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     {
 #pragma unroll
       for (int r = 0; r < kMaxCluster; ++r)
-        if (r < C) upto += cluster.map_shared_rank(&red, r)->bin[by_mass][lane & (kSplit - 1)];
+        if (r < C) upto += peer(&red.bin[by_mass][lane & (kSplit - 1)], r);
       // at least so many tokens are in the bin: none of them weighs more than its first
       float few = !by_mass || upto == 0.f ? upto : upto / exp2a(-fmaxf((float)(lane & (kSplit - 1)) - 0.5f, 0.f) * w * c2);
 #pragma unroll
@@ -595,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
           const double goal = by_mass ? (double)rest * 4294967296.0 - (double)over : (double)rest - (double)over;
           const int last = max(1, __syncthreads_count(tid < got && (by_mass ? (double)ahead : (double)place) < goal)) - 1;
           if (tid < got && place == last)
-            for (int r = 0; r < C; ++r) cluster.map_shared_rank(&red, r)->cut = me;
+            for (int r = 0; r < C; ++r) peer_set(reinterpret_cast<unsigned long long*>(&red.cut), r, bits_of(me));
         }
         cluster.sync();
         cut = red.cut;
@@ -621,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       if (tid == 0) red.mass = mass;
       cluster.sync();
       mass = 0;
-      for (int r = 0; r < C; ++r) mass += cluster.map_shared_rank(&red, r)->mass;
+      for (int r = 0; r < C; ++r) mass += peer(&red.mass, r);
       goal = min(max((unsigned long long)ceil((double)tp * (double)mass), 1ull), mass);
     }
     int left = KB + ib;  // key bits not fixed yet
@@ -718,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   if (tid == 0) red.best = best;
   cluster.sync();
 #pragma unroll 1
-  for (int r = 0; r < C; ++r) best = max64(best, cluster.map_shared_rank(&red, r)->best);
+  for (int r = 0; r < C; ++r) best = max64(best, peer(&red.best, r));
   if (best == 0) {  // every kept token's quotient is 0 (its noise infinite, negative or NaN): the first of them
     each(least, [&](float v, int i) {
       if (kept(v, i)) best = max64(best, 0xffffffffu - (unsigned)(lo + i));
@@ -728,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     if (tid == 0) red.best = best;
     cluster.sync();
 #pragma unroll 1
-    for (int r = 0; r < C; ++r) best = max64(best, cluster.map_shared_rank(&red, r)->best);
+    for (int r = 0; r < C; ++r) best = max64(best, peer(&red.best, r));
   }
   if (rank == 0 && tid == 0) finish(best);
   cluster.sync();  // the others' shared memory stays until rank 0 has read it
