@@ -690,15 +690,31 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     // division that decides, and the tests of what is kept, run for those only.
     const float* e = noise + lo;
     const bool vec = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
+    auto load_noise = [&](int i, float (&en)[VE]) {
+      if (vec && (i + 1) * VE <= n) {
+#pragma unroll
+        for (int q = 0; q < VE / 4; ++q) {
+          const uint4 b = ld_stream_u4(e + i * VE + 4 * q);
+          en[4 * q] = __uint_as_float(b.x), en[4 * q + 1] = __uint_as_float(b.y);
+          en[4 * q + 2] = __uint_as_float(b.z), en[4 * q + 3] = __uint_as_float(b.w);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) en[j] = i * VE + j < n ? __ldg(e + i * VE + j) : 1.f;
+      }
+    };
     float first = 0.f;  // from each thread's first tokens
     if (tid < nvec) {
+      const uint4 w = *reinterpret_cast<const uint4*>(stage + tid * VE);
+      if (Vec<T>::largest(w) >= least) {
+        T v[VE];
+        float en[VE];
+        memcpy(v, &w, 16);
+        load_noise(tid, en);
 #pragma unroll
-      for (int j = 0; j < VE; ++j) {
-        const int at = tid * VE + j;
-        const float x = to_f<T>(stage[at]) + 0.f;
-        if (at < n && x >= least && kept(x, at)) {
-          const float q = __fdividef(weight(x), __ldg(e + at));
-          if (q < 3e38f) first = fmaxf(first, q);
+        for (int j = 0; j < VE; ++j) {
+          const float x = to_f<T>(v[j]) + 0.f, q = __fdividef(weight(x), en[j]);
+          if (kept(x, tid * VE + j) && q < 3e38f) first = fmaxf(first, q);
         }
       }
     }
@@ -712,30 +728,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       T v[VE];
       memcpy(v, &w, 16);
       float en[VE];
-      if (vec && (i + 1) * VE <= n) {
-#pragma unroll
-        for (int q = 0; q < VE / 4; ++q) {
-          const uint4 b = ld_stream_u4(e + i * VE + 4 * q);
-          en[4 * q] = __uint_as_float(b.x), en[4 * q + 1] = __uint_as_float(b.y);
-          en[4 * q + 2] = __uint_as_float(b.z), en[4 * q + 3] = __uint_as_float(b.w);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < VE; ++j) en[j] = i * VE + j < n ? __ldg(e + i * VE + j) : 1.f;
-      }
+      load_noise(i, en);
       const float lead = __int_as_float(*reinterpret_cast<volatile int*>(&lead_s));
       bool near_lead = false;  // (w / e > lead; a negative or NaN e is no matter here)
 #pragma unroll
       for (int j = 0; j < VE; ++j) near_lead |= weight(to_f<T>(v[j])) > lead * en[j];
       if (!near_lead) continue;
-#pragma unroll 1
+#pragma unroll
       for (int j = 0; j < VE; ++j) {
-        const float x = to_f<T>(stage[i * VE + j]) + 0.f;
+        const float x = to_f<T>(v[j]) + 0.f;
         const int at = i * VE + j;
-        if (at >= n || !kept(x, at)) continue;
-        const unsigned long long cand = ticket(weight(x), __ldg(e + at), lo + at);
-        if (cand >> 32 == 0 || cand <= best) continue;
-        best = cand;
+        if (!(weight(x) > lead * en[j]) || at >= n || !kept(x, at)) continue;
+        const unsigned long long cand = ticket(weight(x), en[j], lo + at);
+        if (cand >> 32 == 0) continue;
         atomicMax(&best_s, cand);
         atomicMax(&lead_s, __float_as_int(fminf(__uint_as_float((uint32_t)(cand >> 32)) * 0.9999f, 3e38f)));
       }
