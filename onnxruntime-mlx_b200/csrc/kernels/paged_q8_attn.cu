@@ -1,25 +1,36 @@
 // Attention of packed query rows over the 8-bit paged KV cache (layout: paged_q8.cuh).
 //
 // For row i of sequence b at position p: s_j = scale <q, K_j> ks_j (q after RoPE, K_j the codes, ks_j
-// their scale), o = sum_j softmax(s)_j vs_j V_j over j = 0 .. p.  Every code is exact in fp16, so both
-// products run on mma.sync.m16n8k16 with fp32 accumulation; ks multiplies the finished score and vs
-// the probability.  With G query heads per kv head a cache byte feeds 2 G multiply-adds, so HBM bounds
-// the kernel while the head group fits one matrix tile.
+// their scale), o = sum_j softmax(s)_j vs_j V_j over j = 0 .. p.  With G query heads per kv head a cache
+// byte feeds 2 G multiply-adds, so HBM bounds it at long contexts: 64 sequences of 8192 keys (32 / 8
+// heads, head size 128, fp16) take 197 us on int8 and 199 us on e4m3 codes, 86 % and 85 % of the copy
+// rate in cache bytes.  Short ragged contexts are bound by what a segment costs to start and end (256
+// rows of 1 to 500 keys: 50 us), one sequence alone by latency (1024 keys: 12 us).
 //
-//   * Keys are the 16 rows of the tile and the query heads its 8 columns (S^T = K Q^T, O^T = V^T P^T):
-//     groups of up to 8 heads fill the tile, where heads as rows would leave half of it empty.  The
-//     score tile becomes the operand of the second product by movmatrix (an 8x8 transpose).
+//   * Products on mma.sync with keys as the 16 rows and the query heads as the 8 columns of a tile
+//     (S^T = K Q^T, O^T = V^T P^T): groups of up to 8 heads fill it, where heads as rows would leave half
+//     of it empty.  The score tile becomes the operand of the second product by movmatrix.  tcgen05 has
+//     64 or 128 rows for these 4 to 16 heads, and takes no operand with a scale per key.
+//   * int8: K Q^T on integer products (m16n8k32), q as two (bf16) or three bytes of a fixed-point number,
+//     exact but for q's last place; the codes go from shared memory straight into the tile.  (Widening
+//     them to fp16 and splitting q in two there: 212 us instead of 197.)  e4m3: codes widened to fp16 by
+//     the conversion instruction (193 us where bit shifts took 280), q as one (bf16) or two fp16 numbers
+//     over a power of two that brings its largest element into [1, 2).
+//   * V widens to fp16 (both kinds of code are exact there), P vs is fp16 over a running power of two of
+//     vs, times 2^kLift (11 bits down to 2^-20 of the largest); fp32 rows carry it as two fp16 numbers.
+//     ks multiplies the finished score.  Sums and statistics are fp32.
+//   * The running maximum moves only when a score passes it by 2^kSlack: most units cost one vote instead
+//     of the shuffles of an exact maximum.
 //   * The contraction order is free, so each thread takes D / 4 consecutive bytes of a key row (and
 //     D / 8 of a value row) with wide shared-memory loads; the query is laid out to match.  No
 //     ldmatrix, which moves 16-bit elements.
-//   * q is divided by a power of two so that its largest element lies in [1, 2) (any input range fits
-//     fp16); P vs is divided by a running power of two of vs and lifted by 2^14 (fp16 keeps 11 bits
-//     down to 2^-28 of the largest).  SPLIT carries q and P as the sum of two fp16 numbers (22 bits),
-//     for fp32 rows.
-//   * Work is cut evenly: the (row, kv head, head chunk, 32-key unit) list of the whole batch, in that
-//     order, is divided into equal runs, one per CTA, so ragged lengths cost nothing.  The 4 warps of a
-//     CTA take its units in turn; each streams its own through kStages shared-memory buffers (16-byte
-//     cp.async, swizzled) and runs ahead over the run's segment borders.
+//   * Work is cut evenly: the list of (row, kv head, head chunk, unit of 16 or 32 keys) of the whole batch
+//     is divided into runs of equal weight, one per CTA, so ragged lengths cost nothing; a segment's start
+//     weighs kOver units (without that the CTAs with many short segments ended last: 256 short rows 74 us
+//     instead of 51).  The 4 warps of a CTA take its units in turn; each streams its own through kStages
+//     shared-memory buffers (16-byte cp.async, swizzled; a unit lies in one page where the block size
+//     allows) and runs ahead over the run's segment borders.  Four CTAs an SM (16 warps): instruction
+//     latency, not bytes in flight, is what they hide (two CTAs of twice the unit: 235 us).
 //   * A segment (the part of one (row, head chunk) within a run) is merged over the warps; a segment
 //     that is not the whole of its row goes to the workspace, and the last CTA to arrive joins the
 //     parts in the order of the keys, so results do not depend on timing.
@@ -590,27 +601,27 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
             }
         } else {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+          for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
-        for (int wb = 0; wb < KW; wb += KV) {
-          uint32_t ka[KV], kb[KV];
-          const int r0 = kt * 16 + g, byte = kbyte<D>(c, wb);
-          lds<KV * 4>(buf + swz<D>(r0, byte >> 4) + (byte & 15), ka);
-          lds<KV * 4>(buf + swz<D>(r0 + 8, byte >> 4) + (byte & 15), kb);
+          for (int wb = 0; wb < KW; wb += KV) {
+            uint32_t ka[KV], kb[KV];
+            const int r0 = kt * 16 + g, byte = kbyte<D>(c, wb);
+            lds<KV * 4>(buf + swz<D>(r0, byte >> 4) + (byte & 15), ka);
+            lds<KV * 4>(buf + swz<D>(r0 + 8, byte >> 4) + (byte & 15), kb);
 #pragma unroll
-          for (int w = 0; w < KV; ++w) {
-            uint32_t a[4];
-            widen<CT>(ka[w], a[0], a[2]);
-            widen<CT>(kb[w], a[1], a[3]);
+            for (int w = 0; w < KV; ++w) {
+              uint32_t a[4];
+              widen<CT>(ka[w], a[0], a[2]);
+              widen<CT>(kb[w], a[1], a[3]);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint32_t b[2 * NQ];
-              lds<8 * NQ>(smem_u32(sm) + C::kQ + ((nt * KW + wb + w) * 32 + lane) * (8 * NQ), b);
+              for (int nt = 0; nt < NT; ++nt) {
+                uint32_t b[2 * NQ];
+                lds<8 * NQ>(smem_u32(sm) + C::kQ + ((nt * KW + wb + w) * 32 + lane) * (8 * NQ), b);
 #pragma unroll
-              for (int t = 0; t < NQ; ++t) mma(s[nt], a, b[2 * t], b[2 * t + 1]);
+                for (int t = 0; t < NQ; ++t) mma(s[nt], a, b[2 * t], b[2 * t + 1]);
+              }
             }
           }
-        }
         }
         // scores in base 2, key g (r = 0) and g + 8 (r = 1), heads 2c and 2c + 1
         float vs[2];
