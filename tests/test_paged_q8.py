@@ -344,6 +344,75 @@ def test_attention(ops, code, dt, H, HK, D, bs, new, past):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,D,half,inter,rotary", [
+    ("f16", 64, 32, 1, True),      # pairs
+    ("bf16", 128, 16, 0, True),    # part of the head rotated
+    ("f16", 64, 12, 0, True),      # cos / sin rows off 16 bytes
+    ("f32", 256, 100, 1, True),
+    ("f16", 128, 64, 0, False),    # no RoPE
+])
+def test_attention_rotary_forms(ops, dt, D, half, inter, rotary):
+    c = Case(np.random.default_rng(half), H=4, HK=2, D=D, bs=16, new=[1, 2], past=[37, 150], dt=dt, code="int8",
+             inter=inter, half=half, rotary=rotary)
+    t = c.cuda()
+    out = run_attention(ops, t, c, True)
+    c.codes = cache_of(t, c)
+    v = np.concatenate([c.values(1, b, n).reshape(-1) for b, n in enumerate(c.total)])
+    assert np.abs(out.double().cpu().numpy() - c.attend()).max() <= bound(dt, v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+def test_rows_off_alignment(ops, dt):
+    """Query, key and value rows that start off a 16-byte boundary, with an odd row stride; scales off one as well."""
+    c = Case(np.random.default_rng(21), H=4, HK=2, D=64, bs=16, new=[1, 1, 1], past=[90, 3, 300], dt=dt, code="e4m3")
+    t = c.cuda()
+    want = {n: t[n].clone() for n in ("kc", "vc", "ks", "vs")}
+    out = ops.paged_attention_quantized(t["q"].contiguous(), t["k"].contiguous(), t["v"].contiguous(), want["kc"],
+                                        want["vc"], want["ks"], want["vs"], t["cum"], t["past"], t["bt"], t["cos"],
+                                        t["sin"], num_heads=4, kv_heads=2)
+    wide = torch.zeros(3, 8 * 64 + 7, dtype=DT[dt], device="cuda")
+    wide[:, 1:8 * 64 + 1] = c.qkv.cuda()
+    q, k, v = wide[:, 1:257], wide[:, 257:385], wide[:, 385:513]
+    shifted = {}
+    for n in ("ks", "vs"):
+        flat = torch.zeros(t[n].numel() + 1, device="cuda")
+        flat[1:] = t[n].reshape(-1)
+        shifted[n] = flat[1:].view(t[n].shape)
+    got = ops.paged_attention_quantized(q, k, v, t["kc"], t["vc"], shifted["ks"], shifted["vs"], t["cum"], t["past"],
+                                        t["bt"], t["cos"], t["sin"], num_heads=4, kv_heads=2)
+    assert torch.equal(out, got)
+    assert torch.equal(want["kc"].view(torch.int8), t["kc"].view(torch.int8))
+    assert torch.equal(torch.nan_to_num(want["ks"]), torch.nan_to_num(shifted["ks"]))
+
+
+@pytest.mark.gpu
+def test_cache_past_32_bit_offsets(ops):
+    """Pages at the end of a cache of more than 2^32 bytes (and rows past 2^25): written, read back, attended to."""
+    HK, D, bs = 4, 256, 32
+    blocks = (1 << 32) // (HK * bs * D) + 40
+    kc = torch.empty(blocks, HK, bs, D, dtype=torch.int8, device="cuda")
+    vc, ks = torch.empty_like(kc), torch.empty(blocks, HK, bs, device="cuda")
+    vs = torch.empty_like(ks)
+    n = 70
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn(n, HK * D, device="cuda", generator=g).half() for _ in range(2))
+    q = torch.randn(n, 2 * HK * D, device="cuda", generator=g).half()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    bt = torch.tensor([[blocks - 1, 0, blocks - 20]], **i32)
+    cum, past = torch.tensor([0, n], **i32), torch.zeros(1, **i32)
+    out = ops.paged_attention_quantized(q, k, v, kc, vc, ks, vs, cum, past, bt, num_heads=2 * HK, kv_heads=HK)
+    kr, vr = ops.paged_kv_dequantize(kc, vc, ks, vs, torch.tensor([n], **i32), bt, cap=n, dtype=torch.float32)
+    for got, src in ((kr, k), (vr, v)):
+        rows = src.float().view(n, HK, D).transpose(0, 1)
+        assert ((got[0] - rows).abs() <= rows.abs().amax(-1, keepdim=True) * (0.5 / 127 + 1e-6)).all()
+    x = q[-1].double().view(HK, 2, D)
+    p = torch.softmax(torch.einsum("hgd,hnd->hgn", x, kr[0].double()) / 16.0, -1)
+    o = torch.einsum("hgn,hnd->hgd", p, vr[0].double()).reshape(-1)
+    assert (out[-1].double() - o).abs().max().item() <= bound("f16", vr.cpu().numpy())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["f16", "f32"])
 def test_attention_many_ragged_rows(ops, dt):
     """More rows than a CTA has threads, lengths from 1 to several units: every kind of split."""
