@@ -3,7 +3,7 @@
 // For row i of sequence b at position p: s_j = scale <q, K_j> ks_j (q after RoPE, K_j the codes, ks_j
 // their scale), o = sum_j softmax(s)_j vs_j V_j over j = 0 .. p.  With G query heads per kv head a cache
 // byte feeds 2 G multiply-adds, so HBM bounds it at long contexts: 64 sequences of 8192 keys (32 / 8
-// heads, head size 128, fp16) take 197 us on int8 and 199 us on e4m3 codes, 86 % and 85 % of the copy
+// heads, head size 128, fp16) take 194 us on int8 and 196 us on e4m3 codes, 87 % and 86 % of the copy
 // rate in cache bytes.  Short ragged contexts are bound by what a segment costs to start and end (256
 // rows of 1 to 500 keys: 50 us), one sequence alone by latency (1024 keys: 12 us).
 //
@@ -13,9 +13,10 @@
 //     64 or 128 rows for these 4 to 16 heads, and takes no operand with a scale per key.
 //   * int8: K Q^T on integer products (m16n8k32), q as two (bf16) or three bytes of a fixed-point number,
 //     exact but for q's last place; the codes go from shared memory straight into the tile.  (Widening
-//     them to fp16 and splitting q in two there: 212 us instead of 197.)  e4m3: codes widened to fp16 by
-//     the conversion instruction (193 us where bit shifts took 280), q as one (bf16) or two fp16 numbers
-//     over a power of two that brings its largest element into [1, 2).
+//     them to fp16 and splitting q in two there: 212 us instead of 197 at that step.)  e4m3: codes widened to fp16 by
+//     the conversion instruction (193 us where bit shifts took 280 at that step; mma on the e4m3 codes themselves, q as
+//     four e4m3 numbers: 244 us), q as one (bf16) or two fp16 numbers over a power of two that brings its
+//     largest element into [1, 2).
 //   * V widens to fp16 (both kinds of code are exact there), P vs is fp16 over a running power of two of
 //     vs, times 2^kLift (11 bits down to 2^-20 of the largest); fp32 rows carry it as two fp16 numbers.
 //     ks multiplies the finished score.  Sums and statistics are fp32.
@@ -821,7 +822,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
             int k = 0;
             if (k0 == 0) take(__ldcg(reinterpret_cast<const float4*>(part_at(0) + hd * D + d)), k++);
             const float* pk = first + (k0 + k) * step + hd * D + d;
-            constexpr int MLP = 8;  // parts on their way at once
+            constexpr int MLP = 6;  // parts on their way at once
 #pragma unroll 1
             for (; k < nk; k += MLP, pk += MLP * step) {
               float4 v[MLP];
