@@ -3,7 +3,7 @@
 // For row i of sequence b at position p: s_j = scale <q, K_j> ks_j (q after RoPE, K_j the codes, ks_j
 // their scale), o = sum_j softmax(s)_j vs_j V_j over j = 0 .. p.  With G query heads per kv head a cache
 // byte feeds 2 G multiply-adds, so HBM bounds it at long contexts: 64 sequences of 8192 keys (32 / 8
-// heads, head size 128, fp16) take 194 us on int8 and 196 us on e4m3 codes, 87 % and 86 % of the copy
+// heads, head size 128, fp16) take 194 us on int8 and 199 us on e4m3 codes, 87 % and 85 % of the copy
 // rate in cache bytes.  Short ragged contexts are bound by what a segment costs to start and end (256
 // rows of 1 to 500 keys: 50 us), one sequence alone by latency (1024 keys: 12 us).
 //
@@ -822,7 +822,28 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
             int k = 0;
             if (k0 == 0) take(__ldcg(reinterpret_cast<const float4*>(part_at(0) + hd * D + d)), k++);
             const float* pk = first + (k0 + k) * step + hd * D + d;
-            constexpr int MLP = 6;  // parts on their way at once
+            if (x + nseg >= run) {
+              // the run's last segment: the buffers of warps 1 to 3 are free and take many parts at once (74 parts
+              // of one long sequence: 13 us by registers alone)
+              constexpr int room = (kWarps - 1) * S * C::kStageBytes / (kThreads * 16), NB = room < 32 ? room : 32;
+              const uint32_t slot_ = smem_u32(sm) + S * C::kStageBytes + tid * 16;
+#pragma unroll 1
+              for (; k < nk; k += NB, pk += NB * step) {
+                const int n = min(NB, nk - k);
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) cp16(slot_ + j * (kThreads * 16), pk + j * step);
+                cp_commit();
+                cp_wait<0>();
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) {
+                  uint32_t u[4];
+                  lds<16>(slot_ + j * (kThreads * 16), u);
+                  take(make_float4(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]),
+                                   __uint_as_float(u[3])), k + j);
+                }
+              }
+            }
+            constexpr int MLP = 6;  // else by registers: parts on their way at once
 #pragma unroll 1
             for (; k < nk; k += MLP, pk += MLP * step) {
               float4 v[MLP];
