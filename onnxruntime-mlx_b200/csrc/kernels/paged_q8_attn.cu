@@ -3,9 +3,9 @@
 // For row i of sequence b at position p: s_j = scale <q, K_j> ks_j (q after RoPE, K_j the codes, ks_j
 // their scale), o = sum_j softmax(s)_j vs_j V_j over j = 0 .. p.  With G query heads per kv head a cache
 // byte feeds 2 G multiply-adds, so HBM bounds it at long contexts: 64 sequences of 8192 keys (32 / 8
-// heads, head size 128, fp16) take 194 us on int8 and 199 us on e4m3 codes, 87 % and 85 % of the copy
+// heads, head size 128, fp16) take 203 us on int8 and e4m3 codes, 83 % of the copy
 // rate in cache bytes.  Short ragged contexts are bound by what a segment costs to start and end (256
-// rows of 1 to 500 keys: 50 us), one sequence alone by latency (1024 keys: 12 us).
+// rows of 1 to 500 keys: 51 us), one sequence alone by latency (1024 keys: 12 us).
 //
 //   * Products on mma.sync with keys as the 16 rows and the query heads as the 8 columns of a tile
 //     (S^T = K Q^T, O^T = V^T P^T): groups of up to 8 heads fill it, where heads as rows would leave half
@@ -18,7 +18,9 @@
 //     four e4m3 numbers: 244 us), q as one (bf16) or two fp16 numbers over a power of two that brings its
 //     largest element into [1, 2).
 //   * V widens to fp16 (both kinds of code are exact there), P vs is fp16 over a running power of two of
-//     vs, times 2^kLift (11 bits down to 2^-20 of the largest); fp32 rows carry it as two fp16 numbers.
+//     vs, times 2^kLift (11 bits down to 2^-20 of the largest).  bf16 rows take it as it is; fp16 and fp32 rows as two
+//     fp16 numbers: one would add as much error again as the fp16 output's own rounding (1.4 times plain fp32's against
+//     64 bits, 1.0 times with two; 194 us against 203).
 //     ks multiplies the finished score.  Sums and statistics are fp32.
 //   * The running maximum moves only when a score passes it by 2^kSlack: most units cost one vote instead
 //     of the shuffles of an exact maximum.
@@ -57,7 +59,7 @@ template <typename T, int D, int CT, int NT>
 struct Cfg {
   static constexpr bool kInt = CT == kI8;  // K Q^T on 8-bit integers: q as kNQ bytes; else q as kNQ fp16 terms
   static constexpr int kNQ = kInt + (std::is_same<T, __nv_bfloat16>::value ? 1 : 2);
-  static constexpr int kNP = std::is_same<T, float>::value ? 2 : 1;          // fp16 terms of P
+  static constexpr int kNP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;  // fp16 terms of P
   static constexpr int kUnit = 16 * NT;  // keys of a unit
   static constexpr int kOver = 8 / NT;   // units that a segment's start and end are counted as
   static constexpr int kHeads = 8 * NT;  // query heads of a CTA
