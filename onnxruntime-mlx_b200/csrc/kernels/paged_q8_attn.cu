@@ -11,16 +11,18 @@
 //     (S^T = K Q^T, O^T = V^T P^T): groups of up to 8 heads fill it, where heads as rows would leave half
 //     of it empty.  The score tile becomes the operand of the second product by movmatrix.  tcgen05 has
 //     64 or 128 rows for these 4 to 16 heads, and takes no operand with a scale per key.
-//   * int8: K Q^T on integer products (m16n8k32), q as two (bf16) or three bytes of a fixed-point number,
+//   * int8: K Q^T on integer products (m16n8k32), q as three bytes of a fixed-point number,
 //     exact but for q's last place; the codes go from shared memory straight into the tile.  (Widening
 //     them to fp16 and splitting q in two there: 212 us instead of 197 at that step.)  e4m3: codes widened to fp16 by
 //     the conversion instruction (193 us where bit shifts took 280 at that step; mma on the e4m3 codes themselves, q as
-//     four e4m3 numbers: 244 us), q as one (bf16) or two fp16 numbers over a power of two that brings its
+//     four e4m3 numbers: 244 us), q as two fp16 numbers over a power of two that brings its
 //     largest element into [1, 2).
 //   * V widens to fp16 (both kinds of code are exact there), P vs is fp16 over a running power of two of
-//     vs, times 2^kLift (11 bits down to 2^-20 of the largest).  bf16 rows take it as it is; fp16 and fp32 rows as two
-//     fp16 numbers: one would add as much error again as the fp16 output's own rounding (1.4 times plain fp32's against
-//     64 bits, 1.0 times with two; 194 us against 203).
+//     vs, times 2^kLift, as two fp16 numbers (22 bits).  One adds as much error again as an fp16 output's own rounding
+//     (1.4 times plain fp32's against 64 bits, 1.0 times with two; 194 us against 203).  RoPE leaves q with more bits than
+//     the rows' type, and an output that averages many values is far smaller than they are, so bf16 rows need the same: q
+//     and P in one fp16 number (q in two bytes) moved 9 to 14 % of their outputs to a neighbouring number, none with two
+//     (64 x 8192: 187 us against 205).
 //     ks multiplies the finished score.  Sums and statistics are fp32.
 //   * The running maximum moves only when a score passes it by 2^kSlack: most units cost one vote instead
 //     of the shuffles of an exact maximum.
@@ -58,8 +60,8 @@ constexpr float kSlack = 8.f;  // a score may pass the running maximum by this m
 template <typename T, int D, int CT, int NT>
 struct Cfg {
   static constexpr bool kInt = CT == kI8;  // K Q^T on 8-bit integers: q as kNQ bytes; else q as kNQ fp16 terms
-  static constexpr int kNQ = kInt + (std::is_same<T, __nv_bfloat16>::value ? 1 : 2);
-  static constexpr int kNP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;  // fp16 terms of P
+  static constexpr int kNQ = kInt ? 3 : 2;
+  static constexpr int kNP = 2;  // fp16 terms of P
   static constexpr int kUnit = 16 * NT;  // keys of a unit
   static constexpr int kOver = 8 / NT;   // units that a segment's start and end are counted as
   static constexpr int kHeads = 8 * NT;  // query heads of a CTA
@@ -490,11 +492,11 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       float mul;  // what q is multiplied by
       if constexpr (C::kInt) {
         // q / amax as an integer of kNQ bytes, each in [-128, 127]
-        constexpr float M = NQ == 3 ? 127.f * 65536.f : 127.f * 256.f;
+        constexpr float M = 127.f * 65536.f;
         const float top = fmaxf(__uint_as_float(amax), 1e-30f);  // (all below: q rounds to 0, as its scores would)
         mul = __fdiv_rn(M, top);
         if (lane % LPH == 0)  // what the sum, in units of the upper two bytes' last place, stands for
-          qscale[h] = finite ? top * base * ((NQ == 3 ? 256.f : 1.f) / M) : __uint_as_float(0x7fc00000u);
+          qscale[h] = finite ? top * base * (256.f / M) : __uint_as_float(0x7fc00000u);
       } else {
         const int ex = min(max((int)(amax >> 23), 1), 253);  // biased exponent
         mul = __uint_as_float((uint32_t)(254 - ex) << 23);
@@ -510,7 +512,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
           uint32_t u[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)  // every byte lifted by 128: no carries between them
-            u[e] = (uint32_t)__float2int_rn(finite ? q[4 * j + e] * mul : 0.f) + (NQ == 3 ? 0x808080u : 0x8080u);
+            u[e] = (uint32_t)__float2int_rn(finite ? q[4 * j + e] * mul : 0.f) + 0x808080u;
 #pragma unroll
           for (int t = 0; t < NQ; ++t) {
             const int bi = NQ - 1 - t;  // the most significant byte first
@@ -522,10 +524,8 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
           const __half2 p0 = __floats2half2_rn(a0, a1), p1 = __floats2half2_rn(a2, a3);
           uint32_t* o = dst + (((h >> 3) * KW + w) * 32 + to) * (2 * NQ);
           o[0] = *reinterpret_cast<const uint32_t*>(&p0), o[1] = *reinterpret_cast<const uint32_t*>(&p1);
-          if constexpr (NQ == 2) {
-            o[2] = half2_bits(a0 - __low2float(p0), a1 - __high2float(p0));
-            o[3] = half2_bits(a2 - __low2float(p1), a3 - __high2float(p1));
-          }
+          o[2] = half2_bits(a0 - __low2float(p0), a1 - __high2float(p0));
+          o[3] = half2_bits(a2 - __low2float(p1), a3 - __high2float(p1));
         }
       }
     }
@@ -598,8 +598,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {  // |sums| <= D 127 128: 2^22 at D = 256, 2^30 after the shift
-              int v = si[nt][0][e] * 256 + si[nt][1][e];
-              if constexpr (NQ == 3) v += (si[nt][2][e] + 128) >> 8;
+              const int v = si[nt][0][e] * 256 + si[nt][1][e] + ((si[nt][2][e] + 128) >> 8);
               s[nt][e] = (float)v;
             }
         } else {
@@ -679,8 +678,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
             }
             const __half2 hi = __floats2half2_rn(p[0], p[1]);
             pf[0][nt][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
-            if constexpr (NP == 2)
-              pf[1][nt][r] = transpose8x8(half2_bits(p[0] - __low2float(hi), p[1] - __high2float(hi)));
+            pf[1][nt][r] = transpose8x8(half2_bits(p[0] - __low2float(hi), p[1] - __high2float(hi)));
           }
         // O^T += V^T P^T
 #pragma unroll
