@@ -3,9 +3,9 @@
 // For row i of sequence b at position p: s_j = scale <q, K_j> ks_j (q after RoPE, K_j the codes, ks_j
 // their scale), o = sum_j softmax(s)_j vs_j V_j over j = 0 .. p.  With G query heads per kv head a cache
 // byte feeds 2 G multiply-adds, so HBM bounds it at long contexts: 64 sequences of 8192 keys (32 / 8
-// heads, head size 128, fp16) take 203 us on int8 and e4m3 codes, 83 % of the copy
+// heads, head size 128, fp16) take 207 us on int8 and 202 us on e4m3 codes, 82 and 84 % of the copy
 // rate in cache bytes.  Short ragged contexts are bound by what a segment costs to start and end (256
-// rows of 1 to 500 keys: 51 us), one sequence alone by latency (1024 keys: 12 us).
+// rows of 1 to 500 keys: 53 us), one sequence alone by latency (1024 keys: 12.5 us).
 //
 //   * Products on mma.sync with keys as the 16 rows and the query heads as the 8 columns of a tile
 //     (S^T = K Q^T, O^T = V^T P^T): groups of up to 8 heads fill it, where heads as rows would leave half
@@ -17,15 +17,18 @@
 //     the conversion instruction (193 us where bit shifts took 280 at that step; mma on the e4m3 codes themselves, q as
 //     four e4m3 numbers: 244 us), q as two fp16 numbers over a power of two that brings its
 //     largest element into [1, 2).
-//   * V widens to fp16 (both kinds of code are exact there), P vs is fp16 over a running power of two of
-//     vs, times 2^kLift, as two fp16 numbers (22 bits).  One adds as much error again as an fp16 output's own rounding
+//   * V widens to fp16 (both kinds of code are exact there).  P vs is held times a power of two, each head's own, that
+//     brings the largest product of a warp's keys so far into [2^kLift, kFull), as two fp16 numbers: 22 bits, and a
+//     smallest step of 2^-31 of that product.  (Of the products, and for each head: a value row of a huge scale takes no
+//     bits from the heads that give its key no weight; with one power for all heads, of the scales alone, the int8 case
+//     took 203 us.)  One adds as much error again as an fp16 output's own rounding
 //     (1.4 times plain fp32's against 64 bits, 1.0 times with two; 194 us against 203).  RoPE leaves q with more bits than
 //     the rows' type, and an output that averages many values is far smaller than they are, so bf16 rows need the same: q
 //     and P in one fp16 number (q in two bytes) moved 9 to 14 % of their outputs to a neighbouring number, none with two
 //     (64 x 8192: 187 us against 205).
 //     ks multiplies the finished score.  Sums and statistics are fp32.
-//   * The running maximum moves only when a score passes it by 2^kSlack: most units cost one vote instead
-//     of the shuffles of an exact maximum.
+//   * The running maximum and the power of two move only when a sum or a product passes its limit: most units cost
+//     one vote instead of the shuffles of exact maxima.
 //   * The contraction order is free, so each thread takes D / 4 consecutive bytes of a key row (and
 //     D / 8 of a value row) with wide shared-memory loads; the query is laid out to match.  No
 //     ldmatrix, which moves 16-bit elements.
@@ -52,10 +55,11 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRowTab = 64;
+constexpr int kRowTab = 48;
 constexpr int kLift = 6;       // P vs is held times 2^kLift
 constexpr float kLow = -1e30f;  // the running maximum before the first key: far below any, and finite
-constexpr float kSlack = 8.f;  // a score may pass the running maximum by this much (in base 2) before it moves
+constexpr float kSlack = 0x1p64f;  // the sum of exp(score - running maximum) may reach this before the maximum moves,
+constexpr float kFull = 16384.f;   // and a product with the value's scale, as it is held, this
 
 template <typename T, int D, int CT, int NT>
 struct Cfg {
@@ -73,8 +77,8 @@ struct Cfg {
   static constexpr int kQBytes = kNQ * NT * (D / 16) * 32 * (kInt ? 4 : 8);
   static constexpr int kMl = kQ + kQBytes;                        // [kWarps][kHeads] (m, l)
   static constexpr int kScale = kMl + kWarps * kHeads * 8;        // [kHeads] score factor
-  static constexpr int kMisc = kScale + kHeads * 4;               // [kWarps] (output factor, buffer)
-  static constexpr int kRaw = kMisc + kWarps * 8;                 // the next segment's q rows, cos and sin row
+  static constexpr int kMisc = kScale + kHeads * 4;               // [kWarps][kHeads] output factor, [kWarps] buffer
+  static constexpr int kRaw = kMisc + kWarps * (kHeads + 1) * 4;  // the next segment's q rows, cos and sin row
   static constexpr int kStatic = 768;                             // (bound on the static shared memory)
 };
 
@@ -227,7 +231,8 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
   const uint32_t ring = smem_u32(sm) + warp * S * C::kStageBytes;
   float2* mls = reinterpret_cast<float2*>(sm + C::kMl);
   float* qscale = reinterpret_cast<float*>(sm + C::kScale);
-  float2* misc = reinterpret_cast<float2*>(sm + C::kMisc);
+  float* factor = reinterpret_cast<float*>(sm + C::kMisc);
+  int* buffer = reinterpret_cast<int*>(factor + kWarps * C::kHeads);
   const int HC = kp.HK * hchunks;
   if (tid == 0) {
     mbar_init(&qbar, 1);
@@ -541,10 +546,10 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) qs[nt][0] = qscale[nt * 8 + 2 * c], qs[nt][1] = qscale[nt * 8 + 2 * c + 1];
     float o[MT][NT][4], m[NT][2], l[NT][2];
-    int E = kLift + 1;  // biased exponent that P vs is relative to
+    float dn[NT][2];  // the power of two that a head's P vs is multiplied by
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = kLow, l[nt][0] = l[nt][1] = 0.f;
+      m[nt][0] = m[nt][1] = kLow, l[nt][0] = l[nt][1] = 0.f, dn[nt][0] = dn[nt][1] = 0x1p126f;
 #pragma unroll
       for (int t = 0; t < MT; ++t) o[t][nt][0] = o[t][nt][1] = o[t][nt][2] = o[t][nt][3] = 0.f;
     }
@@ -626,28 +631,32 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
           }
         }
         // scores in base 2, key g (r = 0) and g + 8 (r = 1), heads 2c and 2c + 1
-        float vs[2];
+        float vs[2], p[NT][4], pv[NT][4], ln[NT][2];
         bool move = false;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const bool on = (valid >> (g + r * 8)) & 1u;
           const float ks = lds_f(sks + (g + r * 8) * 4);
           vs[r] = on ? lds_f(svs + (g + r * 8) * 4) : 0.f;
-          move |= __float_as_uint(vs[r]) >= (uint32_t)(E + 1) << 23;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float v = on ? s[nt][r * 2 + h] * (ks * qs[nt][h]) : -INFINITY;
-              s[nt][r * 2 + h] = v;
-              move |= v > m[nt][h] + kSlack;
+              const int e = r * 2 + h;
+              s[nt][e] = on ? s[nt][e] * (ks * qs[nt][h]) : -INFINITY;
+              p[nt][e] = ex2(s[nt][e] - m[nt][h]);
+              pv[nt][e] = p[nt][e] * (vs[r] * dn[nt][h]);
+              move |= !(pv[nt][e] < kFull);
             }
         }
-        if (__any_sync(0xffffffffu, move)) {  // a larger score, or a larger value scale: rescale what there is
-          const int eu = (int)(__reduce_max_sync(0xffffffffu, max(__float_as_uint(vs[0]), __float_as_uint(vs[1]))) >> 23);
-          const int En = min(max(E, eu), 253);
-          const float back = __uint_as_float((uint32_t)max(127 + E - En, 0) << 23);
-          E = En;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            ln[nt][h] = l[nt][h] + p[nt][h] + p[nt][2 + h];
+            move |= !(ln[nt][h] <= kSlack);
+          }
+        if (__any_sync(0xffffffffu, move)) {  // a larger score, or a larger product: rescale what there is
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -657,28 +666,39 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
               for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
               const float a = ex2(m[nt][h] - mx);
               m[nt][h] = mx;
-              l[nt][h] *= a;
+              // the head's largest product, those of the keys before at their present weight (a NaN is passed over)
+              float most = a * __uint_as_float(((uint32_t)(254 + kLift) << 23) - __float_as_uint(dn[nt][h]));
 #pragma unroll
-              for (int t = 0; t < MT; ++t) o[t][nt][h] *= a * back, o[t][nt][2 + h] *= a * back;
+              for (int r = 0; r < 2; ++r) {
+                p[nt][r * 2 + h] = ex2(s[nt][r * 2 + h] - mx);
+                most = fmaxf(most, p[nt][r * 2 + h] * vs[r]);
+              }
+              ln[nt][h] = l[nt][h] * a + p[nt][h] + p[nt][2 + h];
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+              const int ex = min(max((int)(__float_as_uint(most) >> 23), kLift + 1), 253);
+              const float to = __uint_as_float((uint32_t)(254 + kLift - ex) << 23);  // brings it into [1, 2) 2^kLift
+              // to / dn (where a is not 0, `to` is 2^127 dn at most)
+              const int by = (int)(__float_as_uint(to) - __float_as_uint(dn[nt][h])) + (127 << 23);
+              const float back = a == 0.f ? 0.f : a * __int_as_float(max(by, 0));
+              dn[nt][h] = to;
+#pragma unroll
+              for (int t = 0; t < MT; ++t) o[t][nt][h] *= back, o[t][nt][2 + h] *= back;
+#pragma unroll
+              for (int r = 0; r < 2; ++r) pv[nt][r * 2 + h] = p[nt][r * 2 + h] * vs[r] * to;
             }
         }
-        const float down = __uint_as_float((uint32_t)(254 + kLift - E) << 23);
         // P^T as the second operand
         uint32_t pf[NP][NT][2];
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float p[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              p[h] = ex2(s[nt][r * 2 + h] - m[nt][h]);
-              l[nt][h] += p[h];
-              p[h] *= vs[r] * down;
-            }
-            const __half2 hi = __floats2half2_rn(p[0], p[1]);
+            const float* x = pv[nt] + r * 2;
+            l[nt][r] = ln[nt][r];  // (r: a head, here)
+            const __half2 hi = __floats2half2_rn(x[0], x[1]);
             pf[0][nt][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
-            pf[1][nt][r] = transpose8x8(half2_bits(p[0] - __low2float(hi), p[1] - __high2float(hi)));
+            pf[1][nt][r] = transpose8x8(half2_bits(x[0] - __low2float(hi), x[1] - __high2float(hi)));
           }
         // O^T += V^T P^T
 #pragma unroll
@@ -724,15 +744,16 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], d);
           const int hd = nt * 8 + 2 * c + h;
-          if (g == 0) mls[warp * C::kHeads + hd] = make_float2(m[nt][h], l[nt][h]);
+          if (g == 0) {
+            mls[warp * C::kHeads + hd] = make_float2(m[nt][h], l[nt][h]);
+            factor[warp * C::kHeads + hd] = __uint_as_float((254u << 23) - __float_as_uint(dn[nt][h]));  // 1 / dn
+          }
           if (hd < heads)
 #pragma unroll
             for (int t = 0; t < MT; ++t)
               mg[merge_at<D>(hd, (vbyte<D>(g, t >> 1) >> 1) + (t & 1))] = make_float2(o[t][nt][h], o[t][nt][2 + h]);
         }
-      static_assert(kLift == 6, "the power below");
-      if (lane == 0)
-        misc[warp] = make_float2(__uint_as_float((uint32_t)E << 23) * 0x1p-6f, __int_as_float(freeb));
+      if (lane == 0) buffer[warp] = freeb;
     }
     __syncthreads();
     pdl_wait();  // before anything is written
@@ -752,13 +773,14 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
       const int at2 = merge_at<D>(hd, d / 2), at3 = merge_at<D>(hd, d / 2 + 1);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float2 ml = mls[w * C::kHeads + hd], us = misc[w];
+        const float2 ml = mls[w * C::kHeads + hd];
         const float f = ml.y == 0.f ? 0.f : ex2(ml.x - mm);  // 0: the warp saw no key of this segment (a NaN is not 0)
-        const float2* mg = reinterpret_cast<const float2*>(sm + (w * S + __float_as_int(us.y)) * C::kStageBytes);
+        const float2* mg = reinterpret_cast<const float2*>(sm + (w * S + buffer[w]) * C::kStageBytes);
         ll += ml.y * f;
         if (f != 0.f) {  // (else the buffer holds something else)
           const float2 a = mg[at2], b = mg[at3];
-          acc.x += a.x * (f * us.x), acc.y += a.y * (f * us.x), acc.z += b.x * (f * us.x), acc.w += b.y * (f * us.x);
+          const float ff = f * factor[w * C::kHeads + hd];
+          acc.x += a.x * ff, acc.y += a.y * ff, acc.z += b.x * ff, acc.w += b.y * ff;
         }
       }
       if (whole) {
@@ -790,7 +812,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
         const float* first = kp.part + kf * step;
         auto part_at = [&](int k) { return first + (k ? k * step : step / 2); };
         constexpr int KC = D / 2;  // parts at a time: their (m, l) fit a merge buffer
-        float2* mlb = reinterpret_cast<float2*>(sm + __float_as_int(misc[0].y) * C::kStageBytes);
+        float2* mlb = reinterpret_cast<float2*>(sm + buffer[0] * C::kStageBytes);
 #pragma unroll 1
         for (int e0 = 0; e0 < heads * (D / 4); e0 += kThreads) {
           const int e = e0 + tid;

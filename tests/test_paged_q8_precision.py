@@ -123,6 +123,41 @@ def test_the_bounds_see_mistakes(code, dt, shape):
         assert max(verdict(nearest(exact(c, **mistake)[0], dt), o, b, dt)) > 1, mistake
 
 
+def outlier(dt, code, power):
+    """One value row 2^power times the others, seen by heads 0 to 3 alone: heads 4 to 7 give its key e^-40 and less."""
+    c = Case(np.random.default_rng(power), H=8, HK=1, D=64, bs=16, new=[1], past=[90], dt=dt, code=code, rotary=False)
+    at = 37
+    page, off = c.bt[0, at // 16], at % 16
+    big = np.rint(8 * np.sign(np.random.default_rng(1).standard_normal(64)))
+    c.codes[0][0][page, 0, off] = big * (8 if code == "int8" else 16)  # its key: a row of +-64 (+-128) codes
+    row = c.values(0, 0, 91 - 1)[at, 0]
+    q = c.q.copy()
+    for h in range(8):  # scores of +40 and of -60 and less, on top of the others'
+        q[0, h] = np.float16(0.25) * q[0, h] + (40.0 if h < 4 else -70.0) * 8 / (row @ row) * row
+    c.qkv[:, :8 * 64] = torch.from_numpy(q.reshape(1, -1)).to(DT[dt])
+    c.q = c.qkv.double().numpy()[:, :8 * 64].reshape(1, 8, 64)
+    c.codes[1][1][page, 0, off] *= 2.0 ** power
+    return c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("power", [12, 24, 34])
+def test_a_value_scale_that_other_heads_do_not_see(ops, code, dt, power):
+    """The heads that give the large row no weight lose no bits to it (and those that do hold it)."""
+    c = outlier(dt, code, power)
+    t = c.cuda()
+    got = run_attention(ops, t, c, True).double().cpu().numpy().reshape(1, 8, 64)
+    c.codes = cache_of(t, c)
+    o, b = exact(c)
+    assert np.abs(o[:, 4:]).max() < 8 < 2.0 ** 12 < np.abs(o[:, :4]).max()
+    if dt == "f16":  # (larger than the type's largest number)
+        got, o, b = got[:, 4:], o[:, 4:], b[:, 4:]
+    over, _ = verdict(got, o, b, dt)
+    assert over <= 1, over
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
