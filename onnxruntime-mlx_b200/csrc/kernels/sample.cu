@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   float tp = a.top_p ? __ldg(a.top_p + row) : 1.f;
   float mp = a.min_p ? fminf(__ldg(a.min_p + row), 1.f) : 0.f;
   const bool greedy = !(t0 > 0.f);
-  const float t = greedy ? 1.f : t0;
+  const float t = greedy ? 1.f : fmaxf(t0, 1e-38f);  // (1 / t stays finite)
   if (greedy) k = 0, tp = 1.f, mp = 0.f;
   if (k <= 0 || k > a.vocab) k = a.vocab;
   const bool use_p = tp < 1.f;  // (false for NaN)
@@ -299,6 +299,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   }
   // the race's result; called by one thread of the first CTA, after a barrier that follows red.sum
   auto finish = [&](unsigned long long best) {
+    if (best == 0) {  // (no row comes here: its largest logit is always kept)
+      a.tokens[row] = -1;
+      if (a.logprobs) a.logprobs[row] = -INFINITY;
+      return;
+    }
     const int token = (int)(0xffffffffu - (unsigned)(best & 0xffffffffu));
     a.tokens[row] = token;
     if (a.logprobs) {
