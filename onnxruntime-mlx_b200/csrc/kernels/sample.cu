@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   float tp = a.top_p ? __ldg(a.top_p + row) : 1.f;
   float mp = a.min_p ? fminf(__ldg(a.min_p + row), 1.f) : 0.f;
   const bool greedy = !(t0 > 0.f);
-  const float t = greedy ? 1.f : fmaxf(t0, 1e-38f);  // (1 / t stays finite)
+  const float t = greedy ? 1.f : fminf(fmaxf(t0, 1e-38f), 3.4e38f);  // (1 / t stays finite, and above 0)
   if (greedy) k = 0, tp = 1.f, mp = 0.f;
   if (k <= 0 || k > a.vocab) k = a.vocab;
   const bool use_p = tp < 1.f;  // (false for NaN)
