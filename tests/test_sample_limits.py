@@ -35,9 +35,10 @@ def test_temperatures_near_zero(ops, dt, k, p, m):
 @pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("V", [7, 3001, 50257])
 @pytest.mark.parametrize("k,p,m", [(0, 1.0, 0.0), (40, 1.0, 0.0), (0, 0.25, 0.0), (600, 0.5, 0.0), (0, 1.0, 1.0)])
-def test_infinite_temperature(ops, dt, V, k, p, m):
+@pytest.mark.parametrize("scale", [2.5, 2500.0])
+def test_infinite_temperature(ops, dt, V, k, p, m, scale):
     """All logits above -infinity weigh the same: of the first k in order, the first p of them, then the least noise."""
-    x, e = inputs(4, V, dt, V)
+    x, e = inputs(4, V, dt, V, scale)
     x[1, ::2] = -math.inf
     x[2, 1:] = -math.inf
     f = [torch.full((4,), v, dtype=d, device="cuda") for v, d in (
