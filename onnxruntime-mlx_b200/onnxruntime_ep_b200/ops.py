@@ -346,10 +346,10 @@ def _q8_struct(batch, tokens, heads, pages, cache_type, max_blocks, max_seq, hal
 
 
 def _device(*tensors):
-    """The CUDA device that all of the tensors are on."""
+    """The CUDA device that all of the tensors (None: one that was not given) are on."""
     at = tensors[0].get_device()
     for t in tensors:
-        if t.get_device() != at or at < 0:
+        if t is not None and t.get_device() != at or at < 0:
             raise ValueError("the tensors must be on one CUDA device")
     return at
 
@@ -372,7 +372,7 @@ def paged_kv_quantize(key, value, key_cache, value_cache, key_scales, value_scal
     p = _q8_struct(batch, T, 0, pages, _CACHE[key_cache.dtype], block_table.numel() // batch if batch else 1, max_seq,
                    half, interleaved, 0.0, strides)
     device = _device(key, value, key_cache, value_cache, key_scales, value_scales, cumulative_seqlens, past_seqlens,
-                     block_table)
+                     block_table, cos_cache, sin_cache)
     check(L.b200ep_paged_kv_quantize(
         p, key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
         value_scales.data_ptr(), cumulative_seqlens.data_ptr(), past_seqlens.data_ptr(), block_table.data_ptr(),
@@ -437,15 +437,13 @@ def paged_attention_quantized(query, key, value, key_cache, value_cache, key_sca
     strides = _q8_rows("query", query, num_heads * D, dtype, T)
     if key is None and value is None:
         strides = (strides, 0, 0)
-        device = _device(query, key_cache, value_cache, key_scales, value_scales, cumulative_seqlens, past_seqlens,
-                         block_table)
     else:
         if key is None or value is None:
             _q8_fail("key and value come together, or neither")
         strides = (strides, _q8_rows("key", key, kv_heads * D, dtype, T),
                    _q8_rows("value", value, kv_heads * D, dtype, T))
-        device = _device(query, key_cache, value_cache, key_scales, value_scales, cumulative_seqlens, past_seqlens,
-                         block_table, key, value)
+    device = _device(query, key_cache, value_cache, key_scales, value_scales, cumulative_seqlens, past_seqlens,
+                     block_table, key, value, cos_cache, sin_cache, out, workspace)
     if out is None:
         out = torch.empty((T, num_heads * D), dtype=dtype, device=query.device)
     elif out.shape != (T, num_heads * D) or out.dtype != dtype or not out.is_contiguous():
@@ -494,7 +492,7 @@ def sample(logits, noise, temperature=None, top_k=None, top_p=None, min_p=None, 
         raise ValueError(f"sample: tokens must be contiguous int64 with {B} entries")
     if logprobs is not None and (logprobs.dtype != f32 or logprobs.shape != (B,) or not logprobs.is_contiguous()):
         raise ValueError(f"sample: logprobs must be contiguous float32 [{B}]")
-    device = _device(logits, noise)
+    device = _device(logits, noise, temperature, top_k, top_p, min_p, tokens, logprobs)
     if tokens is None:
         tokens = torch.empty(B, dtype=torch.int64, device=logits.device)
     if logprobs is None:

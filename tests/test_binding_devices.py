@@ -1,0 +1,91 @@
+"""Where the tensors of the 8-bit cache's and the sampling bindings may be.  No GPU and no launch: the tensors are on
+the host, get_device() says what the test wants, and the library is a stand-in that counts its calls."""
+
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+I32 = torch.int32
+
+
+class Library:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        if name.endswith("workspace_size"):
+            return lambda *a: 256
+
+        def entry(*a):
+            self.calls.append(name)
+            return 0
+
+        return entry
+
+
+@pytest.fixture
+def world(monkeypatch):
+    """(ops, library, places): places maps a tensor's address to its device, 0 where it is absent."""
+    from onnxruntime_ep_b200 import ops
+
+    ops._lib()
+    library, places = Library(), {}
+    monkeypatch.setattr(ops, "_lib", lambda: library)
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 0)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: places.get(t.data_ptr(), 0))
+    return ops, library, places
+
+
+def cache():
+    return dict(key_cache=torch.zeros(4, 2, 8, 64, dtype=torch.int8), value_cache=torch.zeros(4, 2, 8, 64, dtype=torch.int8),
+                key_scales=torch.zeros(4, 2, 8), value_scales=torch.zeros(4, 2, 8))
+
+
+def tables():
+    return dict(cumulative_seqlens=torch.tensor([0, 1, 2], dtype=I32), past_seqlens=torch.zeros(2, dtype=I32),
+                block_table=torch.zeros(2, 2, dtype=I32), cos_cache=torch.zeros(9, 32).half(),
+                sin_cache=torch.zeros(9, 32).half())
+
+
+def rows(*heads):
+    return [torch.zeros(2, n * 64).half() for n in heads]
+
+
+def arguments(name):
+    if name == "paged_kv_quantize":
+        return dict(zip(("key", "value"), rows(2, 2)), **cache(), **tables()), {}
+    if name == "paged_kv_dequantize":
+        return dict(cache(), seqlens=torch.zeros(2, dtype=I32), block_table=torch.zeros(2, 2, dtype=I32),
+                    key=torch.zeros(2, 2, 5, 64).half(), value=torch.zeros(2, 2, 5, 64).half()), {}
+    if name == "paged_attention_quantized":
+        q, k, v, out = rows(4, 2, 2, 4)
+        return dict(cache(), query=q, key=k, value=v, out=out, workspace=torch.zeros(256, dtype=torch.uint8),
+                    **tables()), dict(num_heads=4, kv_heads=2)
+    return dict(logits=torch.zeros(2, 8), noise=torch.ones(2, 8), temperature=torch.ones(2), top_k=torch.ones(2, dtype=I32),
+                top_p=torch.ones(2), min_p=torch.ones(2), tokens=torch.zeros(2, dtype=torch.int64),
+                logprobs=torch.zeros(2)), {}
+
+
+NAMES = ["paged_kv_quantize", "paged_kv_dequantize", "paged_attention_quantized", "sample"]
+
+
+@pytest.mark.parametrize("name,which", [(n, w) for n in NAMES for w in arguments(n)[0]])
+@pytest.mark.parametrize("place", [-1, 1])
+def test_every_tensor_must_be_on_the_device(world, name, which, place):
+    """Each tensor in turn on the host or on another GPU: refused before any launch."""
+    ops, library, places = world
+    tensors, other = arguments(name)
+    places[tensors[which].data_ptr()] = place
+    with pytest.raises(ValueError, match="one CUDA device"):
+        getattr(ops, name)(**tensors, **other)
+    assert not library.calls
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tensors_on_one_device_are_taken(world, name):
+    ops, library, _ = world
+    tensors, other = arguments(name)
+    getattr(ops, name)(**tensors, **other)
+    assert library.calls == ["b200ep_" + name]
