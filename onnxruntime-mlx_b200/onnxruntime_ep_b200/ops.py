@@ -294,8 +294,8 @@ def _q8_cache(key_cache, value_cache, key_scales, value_scales, block_table, bat
     if not (key_cache.is_contiguous() and value_cache.is_contiguous() and key_scales.is_contiguous()
             and value_scales.is_contiguous()):
         _q8_fail("caches and scales must be contiguous")
-    if block_table.dtype != torch.int32 or not block_table.is_contiguous() or (
-            batch and block_table.numel() % batch):
+    if block_table.dtype != torch.int32 or not block_table.is_contiguous() or batch and (
+            block_table.numel() % batch or block_table.dim() > 1 and block_table.shape[0] != batch):
         _q8_fail("block_table must be a contiguous int32 [batch, max_blocks]")
     return shape
 

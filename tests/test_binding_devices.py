@@ -1,5 +1,5 @@
-"""Where the tensors of the 8-bit cache's and the sampling bindings may be.  No GPU and no launch: the tensors are on
-the host, get_device() says what the test wants, and the library is a stand-in that counts its calls."""
+"""Where the tensors of the 8-bit cache's and the sampling bindings may be, and their shapes.  No GPU and no launch: the
+tensors are on the host, get_device() says what the test wants, and the library is a stand-in that counts its calls."""
 
 from __future__ import annotations
 
@@ -89,3 +89,15 @@ def test_tensors_on_one_device_are_taken(world, name):
     tensors, other = arguments(name)
     getattr(ops, name)(**tensors, **other)
     assert library.calls == ["b200ep_" + name]
+
+
+@pytest.mark.parametrize("name", NAMES[:3])
+@pytest.mark.parametrize("shape", [(4, 2), (1, 4), (4, 1, 2)])
+def test_a_block_table_of_other_sequences_is_refused(world, name, shape):
+    """A pool's table with more rows than there are sequences: its rows would be read as halves of others."""
+    ops, library, _ = world
+    tensors, other = arguments(name)
+    tensors["block_table"] = torch.zeros(shape, dtype=I32)
+    with pytest.raises(ValueError, match="block_table"):
+        getattr(ops, name)(**tensors, **other)
+    assert not library.calls
