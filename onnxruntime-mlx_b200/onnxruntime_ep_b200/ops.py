@@ -453,6 +453,8 @@ def paged_attention_quantized(query, key, value, key_cache, value_cache, key_sca
     if workspace is None:
         workspace = torch.empty(L.b200ep_paged_attention_quantized_workspace_size(p), dtype=torch.uint8,
                                 device=query.device)
+    elif not workspace.is_contiguous():
+        _q8_fail("workspace must be contiguous")
     check(L.b200ep_paged_attention_quantized(
         p, query.data_ptr(), key if key is None else key.data_ptr(), value if value is None else value.data_ptr(),
         key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),

@@ -101,3 +101,12 @@ def test_a_block_table_of_other_sequences_is_refused(world, name, shape):
     with pytest.raises(ValueError, match="block_table"):
         getattr(ops, name)(**tensors, **other)
     assert not library.calls
+
+
+def test_a_workspace_that_is_smaller_than_its_size_says_is_refused(world):
+    ops, library, _ = world
+    tensors, other = arguments("paged_attention_quantized")
+    tensors["workspace"] = torch.zeros(1, dtype=torch.uint8).expand(1 << 20)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.paged_attention_quantized(**tensors, **other)
+    assert not library.calls
