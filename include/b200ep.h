@@ -286,8 +286,9 @@ B200EP_API int b200ep_paged_attention_quantized(
  * of these, those with w_j >= min_p; always the first.  The token is the kept one with the largest
  * w_j / noise_j (ties: lowest index): for noise of independent standard exponential numbers (float32
  * [rows, vocab], > 0) that is a draw from the kept tokens' distribution.
- *   temperature [rows]: 0 takes the first token (NULL: 1), below 1e-38 it counts as 1e-38,
- *   infinity weighs all logits above -infinity alike;  top_k int32 [rows]: <= 0 keeps all (NULL);  top_p [rows]: >= 1 keeps all (NULL);  min_p [rows]: <= 0 keeps all (NULL)
+ *   temperature [rows]: 0 takes the first token (NULL: 1), below 1e-38 it counts as 1e-38, infinity weighs all logits
+ *   above -infinity alike;  top_k int32 [rows]: <= 0 keeps all (NULL);  top_p [rows]: >= 1 keeps all (NULL);
+ *   min_p [rows]: <= 0 keeps all (NULL)
  *   tokens int64 [rows]: -1 for a row without a logit above -infinity;  logprobs float32 [rows] (may be
  *   NULL): log softmax of the logits as given, at the token
  * NaN logits are never taken.  Equal inputs give equal tokens.  vocab up to 262144. */

@@ -358,6 +358,20 @@ def _raw_stream(device):
     return torch._C._cuda_getCurrentRawStream(device)
 
 
+def _current_device():
+    return torch._C._cuda_getDevice()
+
+
+def _launch(device, entry, *args):
+    """Calls an entry point on the device's current stream (its last argument).  It launches on the current device, so
+    the tensors' is made that one."""
+    if _current_device() == device:
+        check(entry(*args, _raw_stream(device)))
+    else:
+        with torch.cuda.device(device):
+            check(entry(*args, _raw_stream(device)))
+
+
 def paged_kv_quantize(key, value, key_cache, value_cache, key_scales, value_scales, cumulative_seqlens,
                       past_seqlens, block_table, cos_cache=None, sin_cache=None, *, interleaved=0):
     """Write packed key / value rows [T, kv_heads * D] (the key after RoPE) into 8-bit pages, in place:
@@ -373,10 +387,11 @@ def paged_kv_quantize(key, value, key_cache, value_cache, key_scales, value_scal
                    half, interleaved, 0.0, strides)
     device = _device(key, value, key_cache, value_cache, key_scales, value_scales, cumulative_seqlens, past_seqlens,
                      block_table, cos_cache, sin_cache)
-    check(L.b200ep_paged_kv_quantize(
-        p, key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
-        value_scales.data_ptr(), cumulative_seqlens.data_ptr(), past_seqlens.data_ptr(), block_table.data_ptr(),
-        half and cos_cache.data_ptr(), half and sin_cache.data_ptr(), _TYPE.get(dtype, 0), _raw_stream(device)))
+    _launch(
+        device, L.b200ep_paged_kv_quantize, p, key.data_ptr(), value.data_ptr(), key_cache.data_ptr(),
+        value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), cumulative_seqlens.data_ptr(),
+        past_seqlens.data_ptr(), block_table.data_ptr(), half and cos_cache.data_ptr(), half and sin_cache.data_ptr(),
+        _TYPE.get(dtype, 0))
 
 
 def paged_kv_dequantize(key_cache, value_cache, key_scales, value_scales, seqlens, block_table, *, cap=None,
@@ -406,10 +421,10 @@ def paged_kv_dequantize(key_cache, value_cache, key_scales, value_scales, seqlen
         device = _device(key_cache, value_cache, key_scales, value_scales, seqlens, block_table, key, value)
     p = _q8_struct(B, 0, 0, pages, _CACHE[key_cache.dtype], block_table.numel() // B if B else 1, 0, 0, 0, 0.0,
                    (0, 0, 0))
-    check(L.b200ep_paged_kv_dequantize(
-        p, key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
-        seqlens.data_ptr(), block_table.data_ptr(), key.data_ptr(), value.data_ptr(), cap, _TYPE.get(key.dtype, 0),
-        _raw_stream(device)))
+    _launch(
+        device, L.b200ep_paged_kv_dequantize, p, key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+        value_scales.data_ptr(), seqlens.data_ptr(), block_table.data_ptr(), key.data_ptr(), value.data_ptr(), cap,
+        _TYPE.get(key.dtype, 0))
     return key, value
 
 
@@ -455,12 +470,13 @@ def paged_attention_quantized(query, key, value, key_cache, value_cache, key_sca
                                 device=query.device)
     elif not workspace.is_contiguous():
         _q8_fail("workspace must be contiguous")
-    check(L.b200ep_paged_attention_quantized(
-        p, query.data_ptr(), key if key is None else key.data_ptr(), value if value is None else value.data_ptr(),
+    _launch(
+        device, L.b200ep_paged_attention_quantized, p, query.data_ptr(), key if key is None else key.data_ptr(),
+        value if value is None else value.data_ptr(),
         key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
         cumulative_seqlens.data_ptr(), past_seqlens.data_ptr(), block_table.data_ptr(),
         half and cos_cache.data_ptr(), half and sin_cache.data_ptr(), out.data_ptr(), _TYPE.get(dtype, 0),
-        workspace.data_ptr(), workspace.nbytes, _raw_stream(device)))
+        workspace.data_ptr(), workspace.nbytes)
     return out
 
 
@@ -499,6 +515,6 @@ def sample(logits, noise, temperature=None, top_k=None, top_p=None, min_p=None, 
         tokens = torch.empty(B, dtype=torch.int64, device=logits.device)
     if logprobs is None:
         logprobs = torch.empty(B, dtype=f32, device=logits.device)
-    check(L.b200ep_sample(logits.data_ptr(), noise.data_ptr(), *args, tokens.data_ptr(), logprobs.data_ptr(), B, V,
-                          lr if B > 1 else 0, nr if B > 1 else 0, _TYPE.get(logits.dtype, 0), _raw_stream(device)))
+    _launch(device, L.b200ep_sample, logits.data_ptr(), noise.data_ptr(), *args, tokens.data_ptr(), logprobs.data_ptr(),
+            B, V, lr if B > 1 else 0, nr if B > 1 else 0, _TYPE.get(logits.dtype, 0))
     return tokens, logprobs

@@ -34,13 +34,14 @@ def world(monkeypatch):
     library, places = Library(), {}
     monkeypatch.setattr(ops, "_lib", lambda: library)
     monkeypatch.setattr(ops, "_raw_stream", lambda device: 0)
+    monkeypatch.setattr(ops, "_current_device", lambda: 0)
     monkeypatch.setattr(torch.Tensor, "get_device", lambda t: places.get(t.data_ptr(), 0))
     return ops, library, places
 
 
 def cache():
-    return dict(key_cache=torch.zeros(4, 2, 8, 64, dtype=torch.int8), value_cache=torch.zeros(4, 2, 8, 64, dtype=torch.int8),
-                key_scales=torch.zeros(4, 2, 8), value_scales=torch.zeros(4, 2, 8))
+    codes = [torch.zeros(4, 2, 8, 64, dtype=torch.int8) for _ in range(2)]
+    return dict(key_cache=codes[0], value_cache=codes[1], key_scales=torch.zeros(4, 2, 8), value_scales=torch.zeros(4, 2, 8))
 
 
 def tables():
@@ -63,8 +64,8 @@ def arguments(name):
         q, k, v, out = rows(4, 2, 2, 4)
         return dict(cache(), query=q, key=k, value=v, out=out, workspace=torch.zeros(256, dtype=torch.uint8),
                     **tables()), dict(num_heads=4, kv_heads=2)
-    return dict(logits=torch.zeros(2, 8), noise=torch.ones(2, 8), temperature=torch.ones(2), top_k=torch.ones(2, dtype=I32),
-                top_p=torch.ones(2), min_p=torch.ones(2), tokens=torch.zeros(2, dtype=torch.int64),
+    return dict(logits=torch.zeros(2, 8), noise=torch.ones(2, 8), temperature=torch.ones(2),
+                top_k=torch.ones(2, dtype=I32), top_p=torch.ones(2), min_p=torch.ones(2), tokens=torch.zeros(2, dtype=torch.int64),
                 logprobs=torch.zeros(2)), {}
 
 
@@ -110,3 +111,29 @@ def test_a_workspace_that_is_smaller_than_its_size_says_is_refused(world):
     with pytest.raises(ValueError, match="contiguous"):
         ops.paged_attention_quantized(**tensors, **other)
     assert not library.calls
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_the_launch_is_on_the_tensors_device(world, monkeypatch, name):
+    """Tensors on a device that is not the current one: it is current while the entry point runs, and not after."""
+    ops, library, places = world
+    tensors, other = arguments(name)
+    for x in tensors.values():
+        places[x.data_ptr()] = 3
+    now, seen = [0], []
+
+    class device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.index
+
+        def __exit__(self, *a):
+            now[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(ops, "_current_device", lambda: now[0])
+    setattr(library, "b200ep_" + name, lambda *a: seen.append(now[0]) or 0)
+    getattr(ops, name)(**tensors, **other)
+    assert seen == [3] and now == [0]
