@@ -276,8 +276,8 @@ __global__ void __launch_bounds__(kReadThreads) paged_q8_read_kernel(PagedQ8Read
     for (int q = 0; q < 4; ++q) {
       uint32_t h01, h23;
       widen<CT>(c[q], h01, h23);
-      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h01));
-      const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&h23));
+      const float2 a = __half22float2(half2_of(h01));
+      const float2 d = __half22float2(half2_of(h23));
       y[4 * q] = from_f<T>(zero ? 0.f : a.x * scale), y[4 * q + 1] = from_f<T>(zero ? 0.f : a.y * scale);
       y[4 * q + 2] = from_f<T>(zero ? 0.f : d.x * scale), y[4 * q + 3] = from_f<T>(zero ? 0.f : d.y * scale);
     }

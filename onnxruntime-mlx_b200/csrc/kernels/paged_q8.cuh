@@ -7,6 +7,8 @@
 // reads block_size * head_size contiguous bytes per page.
 #pragma once
 
+#include <cstring>
+
 #include "../common.cuh"
 
 namespace b200ep {
@@ -67,6 +69,18 @@ __device__ __forceinline__ int q8_row(const int32_t* bt, int maxb, int nblocks, 
   return phys < 0 || phys >= nblocks ? -1 : (phys * HK + h) * bs + (pos - blk * bs);
 }
 
+// The bits of two fp16 numbers, and back.
+__device__ __forceinline__ uint32_t word_of(__half2 h) {
+  uint32_t w;
+  memcpy(&w, &h, 4);
+  return w;
+}
+__device__ __forceinline__ __half2 half2_of(uint32_t w) {
+  __half2 h;
+  memcpy(&h, &w, 4);
+  return h;
+}
+
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
 // The four codes of a word as two f16x2 (codes 0, 1 and 2, 3).
@@ -76,9 +90,8 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& h01, uint32_t& h23) 
     // 0x6400 | (code + 128) is 1024 + 128 + code in fp16
     const uint32_t x = w ^ 0x80808080u;
     const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    uint32_t a = prmt(x, 0x64646464u, 0x4140), b = prmt(x, 0x64646464u, 0x4342);
-    __half2 ha = __hsub2(*reinterpret_cast<__half2*>(&a), bias), hb = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
-    h01 = *reinterpret_cast<uint32_t*>(&ha), h23 = *reinterpret_cast<uint32_t*>(&hb);
+    h01 = word_of(__hsub2(half2_of(prmt(x, 0x64646464u, 0x4140)), bias));
+    h23 = word_of(__hsub2(half2_of(prmt(x, 0x64646464u, 0x4342)), bias));
   } else {
     asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
         : "=r"(h01), "=r"(h23) : "r"(w));

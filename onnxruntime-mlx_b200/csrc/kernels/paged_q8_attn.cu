@@ -131,8 +131,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
-  __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&h);
+  return word_of(__floats2half2_rn(lo, hi));
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -528,7 +527,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
           const float a0 = q[4 * j] * mul, a1 = q[4 * j + 1] * mul, a2 = q[4 * j + 2] * mul, a3 = q[4 * j + 3] * mul;
           const __half2 p0 = __floats2half2_rn(a0, a1), p1 = __floats2half2_rn(a2, a3);
           uint32_t* o = dst + (((h >> 3) * KW + w) * 32 + to) * (2 * NQ);
-          o[0] = *reinterpret_cast<const uint32_t*>(&p0), o[1] = *reinterpret_cast<const uint32_t*>(&p1);
+          o[0] = word_of(p0), o[1] = word_of(p1);
           o[2] = half2_bits(a0 - __low2float(p0), a1 - __high2float(p0));
           o[3] = half2_bits(a2 - __low2float(p1), a3 - __high2float(p1));
         }
@@ -697,7 +696,7 @@ paged_q8_attn_kernel(PagedQ8 kp, int hchunks, int appended, int vec) {
             const float* x = pv[nt] + r * 2;
             l[nt][r] = ln[nt][r];  // (r: a head, here)
             const __half2 hi = __floats2half2_rn(x[0], x[1]);
-            pf[0][nt][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
+            pf[0][nt][r] = transpose8x8(word_of(hi));
             pf[1][nt][r] = transpose8x8(half2_bits(x[0] - __low2float(hi), x[1] - __high2float(hi)));
           }
         // O^T += V^T P^T

@@ -103,6 +103,18 @@ __device__ __forceinline__ unsigned long long fixed32(float w) {  // w in [0, 1]
   return ((unsigned long long)(uint32_t)hi << 16) + (unsigned long long)__float2uint_rn((h - hi) * 65536.f);
 }
 
+// 16 bytes of the slice, at a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ uint4 get16(const T* p) {
+  uint4 w;
+  memcpy(&w, __builtin_assume_aligned(p, 16), 16);
+  return w;
+}
+template <typename T>
+__device__ __forceinline__ void put16(T* p, const uint4& w) {
+  memcpy(__builtin_assume_aligned(p, 16), &w, 16);
+}
+
 // 16 bytes of logits: NaN to -infinity, and the largest.
 template <typename T>
 struct Vec;
@@ -233,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     for (int i = tid; i < n / VE; i += kThreads) {
       uint4 w = ld_stream_u4(g + i * VE);
       mine = fmaxf(mine, Vec<T>::clean(w));
-      *reinterpret_cast<uint4*>(stage + i * VE) = w;
+      put16(stage + i * VE, w);
     }
   }
 #pragma unroll 1
@@ -247,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   auto each = [&](float least, auto f) {
 #pragma unroll 1
     for (int i = tid; i < nvec; i += kThreads) {
-      const uint4 w = *reinterpret_cast<const uint4*>(stage + i * VE);
+      const uint4 w = get16(stage + i * VE);
       if (Vec<T>::largest(w) < least) continue;
       T v[VE];
       memcpy(v, &w, 16);
@@ -582,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
 #pragma unroll 1
       for (int i0 = warp * 32; i0 < nvec; i0 += kThreads) {
         const int i = i0 + lane;
-        const uint4 w4 = i < nvec ? *reinterpret_cast<const uint4*>(stage + i * VE) : uint4{};
+        const uint4 w4 = i < nvec ? get16(stage + i * VE) : uint4{};
         T v[VE];
         memcpy(v, &w4, 16);
         uint32_t in = 0;  // which of the thread's VE tokens
@@ -713,7 +725,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     };
     float first = 0.f;  // from each thread's first tokens
     if (tid < nvec) {
-      const uint4 w = *reinterpret_cast<const uint4*>(stage + tid * VE);
+      const uint4 w = get16(stage + tid * VE);
       if (Vec<T>::largest(w) >= least) {
         T v[VE];
         float en[VE];
@@ -731,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     __syncthreads();
 #pragma unroll 1
     for (int i = tid; i < nvec; i += kThreads) {
-      const uint4 w = *reinterpret_cast<const uint4*>(stage + i * VE);
+      const uint4 w = get16(stage + i * VE);
       if (Vec<T>::largest(w) < least) continue;
       T v[VE];
       memcpy(v, &w, 16);
