@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   uint32_t* mhi = mlo + kBins;
   T* stage = reinterpret_cast<T*>(mhi + kBins);
   __shared__ Red red;
-  __shared__ unsigned long long seg_s[2][2];    // histograms: this CTA's share
+  __shared__ unsigned long long seg_s[2];       // histograms: this CTA's share
   __shared__ unsigned long long found_s[2][4];  // the bin found: flag, bin, before it, its count
   __shared__ unsigned long long scratch[kWarpsS];
   __shared__ int top_s, lead_s;
@@ -477,12 +477,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       total += scratch[w];
     }
     const int par = round++ & 1;
-    if (tid == 0) seg_s[par][0] = total, found_s[par][0] = 0;
+    if (tid == 0) seg_s[par] = total, found_s[par][0] = 0;
     cluster.sync();
     unsigned long long sum = 0;
 #pragma unroll
     for (int r = 0; r < kMaxCluster; ++r) {
-      const unsigned long long v = r < C ? peer(&seg_s[par][0], r) : 0;
+      const unsigned long long v = r < C ? peer(&seg_s[par], r) : 0;
       if (r < rank) ahead_ += v;
       sum += v;
     }
