@@ -2,10 +2,11 @@
 //
 // For row i of sequence b at position p: s_j = scale <q, K_j> ks_j (q after RoPE, K_j the codes, ks_j
 // their scale), o = sum_j softmax(s)_j vs_j V_j over j = 0 .. p.  With G query heads per kv head a cache
-// byte feeds 2 G multiply-adds, so HBM bounds it at long contexts: 64 sequences of 8192 keys (32 / 8
+// byte feeds 2 G multiply-adds, so HBM should bound it at long contexts: 64 sequences of 8192 keys (32 / 8
 // heads, head size 128, fp16) take 207 us on int8 and 202 us on e4m3 codes, 82 and 84 % of the copy
-// rate in cache bytes.  Short ragged contexts are bound by what a segment costs to start and end (256
-// rows of 1 to 500 keys: 53 us), one sequence alone by latency (1024 keys: 12.5 us).
+// rate in cache bytes, at 1965 MHz; its instructions are as near a bound: back to back for longer the power cap holds
+// 1.69 GHz, and the time follows the clock (230 us).  Short ragged contexts are bound by what a segment costs to start
+// and end (256 rows of 1 to 500 keys: 52 us), one sequence alone by latency (1024 keys: 12.4 us).
 //
 //   * Products on mma.sync with keys as the 16 rows and the query heads as the 8 columns of a tile
 //     (S^T = K Q^T, O^T = V^T P^T): groups of up to 8 heads fill it, where heads as rows would leave half
