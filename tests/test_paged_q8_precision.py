@@ -68,7 +68,7 @@ def exact(c, scale=None, p_bits=None, q_bits=None, drop=None):
     return out, b
 
 
-def verdict(got, o, b, dt):
+def excess(got, o, b, dt):
     """(most that an element is off over what it may be, flipped elements over what they may be)"""
     step = last_place(o, dt)
     over = (np.abs(got - o) / (step / 2 + 8 * b + 1e-300)).max()
@@ -103,7 +103,7 @@ def test_elements(ops, code, dt, shape):
     got = run_attention(ops, t, c, True).double().cpu().numpy().reshape(c.T, c.H, c.D)
     c.codes = cache_of(t, c)
     o, b = exact(c)
-    over, flips = verdict(got, o, b, dt)
+    over, flips = excess(got, o, b, dt)
     assert over <= 1, over
     if dt != "f32":  # (32-bit outputs have no room below their own rounding)
         assert flips <= 1, flips
@@ -117,10 +117,10 @@ def test_the_bounds_see_mistakes(code, dt, shape):
     c = made(*shape, dt, code)
     c.put(c.written())
     o, b = exact(c)
-    assert max(verdict(nearest(o, dt), o, b, dt)) <= 1
+    assert max(excess(nearest(o, dt), o, b, dt)) <= 1
     n = max(c.total)
     for mistake in (dict(drop=(n - 16, n)), dict(q_bits=11), dict(p_bits=11)):
-        assert max(verdict(nearest(exact(c, **mistake)[0], dt), o, b, dt)) > 1, mistake
+        assert max(excess(nearest(exact(c, **mistake)[0], dt), o, b, dt)) > 1, mistake
 
 
 def outlier(dt, code, power):
@@ -154,7 +154,7 @@ def test_a_value_scale_that_other_heads_do_not_see(ops, code, dt, power):
     assert np.abs(o[:, 4:]).max() < 8 < 2.0 ** 12 < np.abs(o[:, :4]).max()
     if dt == "f16":  # (larger than the type's largest number)
         got, o, b = got[:, 4:], o[:, 4:], b[:, 4:]
-    over, _ = verdict(got, o, b, dt)
+    over, _ = excess(got, o, b, dt)
     assert over <= 1, over
 
 
@@ -169,7 +169,7 @@ def test_elements_of_a_long_sequence(ops, code, dt, H, HK, D):
     got = run_attention(ops, t, c, True).double().cpu().numpy().reshape(c.T, c.H, c.D)
     c.codes = cache_of(t, c)
     o, b = exact(c)
-    over, _ = verdict(got, o, b, dt)
+    over, _ = excess(got, o, b, dt)
     assert over <= 1, over
 
 
@@ -182,5 +182,5 @@ def test_elements_of_many_new_rows(ops, dt):
     got = run_attention(ops, t, c, True).double().cpu().numpy().reshape(c.T, c.H, c.D)
     c.codes = cache_of(t, c)
     o, b = exact(c)
-    over, flips = verdict(got, o, b, dt)
+    over, flips = excess(got, o, b, dt)
     assert over <= 1 and flips <= 1, (over, flips)

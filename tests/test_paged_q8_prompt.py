@@ -16,7 +16,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from test_paged_q8 import Case, _device_error_clean, cache_of, ops, rotate, run_attention  # noqa: E402,F401
-from test_paged_q8_precision import exact, last_place, verdict  # noqa: E402
+from test_paged_q8_precision import exact, last_place, excess  # noqa: E402
 
 H, HK, D, S = 8, 2, 64, 51
 CHUNKS = ((0, 7), (7, 8), (8, 40), (40, 50))
@@ -69,7 +69,7 @@ def test_prompt_in_chunks_and_a_decode_step(ops, code):
                                         torch.tensor([50], **i32), t["bt"], t["cos"], t["sin"], num_heads=H, kv_heads=HK)
     c.codes = cache_of(t, c)
     o, b = exact(c)
-    over, _ = verdict(got.double().cpu().numpy().reshape(1, H, D), o[50:], b[50:], "f16")
+    over, _ = excess(got.double().cpu().numpy().reshape(1, H, D), o[50:], b[50:], "f16")
     assert over <= 1, over
 
 
